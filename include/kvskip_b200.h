@@ -292,6 +292,122 @@ int kvskip_launch_append(uint16_t* k, uint16_t* v, int64_t sb, int64_t sh, int64
                          const uint16_t* v_new, int B, int Hkv, int D, int T, const int* t_dev,
                          const int32_t* page_table, int max_pages, int num_pages, void* stream);
 
+/* ---- 8-bit cache (no counterpart in the reference, whose cache is bf16) -----------------------
+ * K and V are held as 8-bit codes with one fp32 scale for every 64-token block and KV head: a value
+ * is code * scale.  kind 0: e4m3 (sign, 4 exponent, 3 mantissa bits; no infinities; largest 448),
+ * kind 1: int8 (codes -127..127).  D is 64 or 128.
+ * Paged form: codes uint8 [num_pages,Hkv,64,D], scales [num_pages,Hkv], a page table; contiguous
+ * form: codes [B,Hkv,T,D], scales [B,Hkv,ceil(T/64)].  D contiguous, all other strides free (code
+ * strides multiples of 16 bytes, 16-byte aligned base).  The entry points are stateless: no memory is
+ * shared between calls, so calls on different streams, and graphs captured from them, are independent
+ * as long as their buffers are. */
+#define KVSKIP_KIND_E4M3 0
+#define KVSKIP_KIND_INT8 1
+
+typedef struct kvskip_decode8_params {
+  const uint16_t* q; /* [B,Hq,D] bf16 or fp16 (q_f16), D contiguous, rows 8-byte aligned */
+  int64_t q_sb, q_sh;
+  const uint8_t* k; /* paged: *_sb is the page stride */
+  const uint8_t* v;
+  int64_t k_sb, k_sh, k_st;
+  int64_t v_sb, v_sh, v_st;
+  const float* k_scale; /* element strides: page or sequence, head, block (contiguous form only) */
+  const float* v_scale;
+  int64_t ks_sb, ks_sh, ks_st;
+  int64_t vs_sb, vs_sh, vs_st;
+  int32_t q_f16, kind;
+  int32_t B, Hq, Hkv, D;
+  int32_t T;                  /* bound on the lengths: it sizes the launch and the statistics rows */
+  float scale_log2;           /* softmax scale * log2(e) */
+  const int32_t* lens;        /* [B] lengths on the device (clamped to [0, T]), or NULL: all T */
+  const int32_t* page_table;  /* [B,max_pages], or NULL: contiguous form */
+  int32_t max_pages, num_pages;
+  const int32_t* block_idx; /* [B,Hkv,max_blocks] ascending, or NULL: every block */
+  const int32_t* block_cnt; /* [B,Hkv] */
+  int32_t max_blocks;
+  int32_t nb;     /* ceil(T / 64): stride of the statistics rows */
+  uint16_t* out;  /* [B,Hq,D] of q's type */
+  float* out_f32; /* optional [B,Hq,D] */
+  float* lse;     /* [B,Hq] natural-log log-sum-exp */
+  float* blk_max; /* optional (both or none) [B,Hq,nb] */
+  float* blk_sum;
+  void* work;     /* kvskip_decode8_work_bytes() bytes, 16-byte aligned, contents irrelevant */
+} kvskip_decode8_params;
+
+/* Attention of one token per sequence over the 8-bit cache, Hq = G * Hkv with 1 <= G <= 16.  Lengths are
+ * read on the device, one per sequence; a sequence of length 0, or a block list without a token, gives
+ * out = 0 and lse = -inf.  Rows of a block behind the length are never used, whatever they hold.  Block
+ * statistics as in kvskip_launch_decode (-inf / 0 on blocks that are not read).  A page table entry
+ * outside the pool reads as zeros; a list entry outside the sequence reads nothing. */
+int64_t kvskip_decode8_work_bytes(int G, int D);
+int kvskip_launch_decode8(const kvskip_decode8_params* p, void* stream);
+
+typedef struct kvskip_write8_params {
+  const uint16_t* k_new; /* token i of n: row (i / inner, i % inner), element strides below, D contiguous */
+  const uint16_t* v_new;
+  int64_t kn_so, kn_si, kn_sh;
+  int64_t vn_so, vn_si, vn_sh;
+  int64_t n, inner;
+  const int64_t* slots; /* [n] slot of every token: block * 64 + row; negative: no slot, the token is skipped */
+  uint8_t* k;
+  uint8_t* v;
+  int64_t k_sb, k_sh, k_st;
+  int64_t v_sb, v_sh, v_st;
+  float* k_scale;
+  float* v_scale;
+  int64_t ks_sb, ks_sh, ks_st;
+  int64_t vs_sb, vs_sh, vs_st;
+  int32_t x_f16, kind;
+  int32_t Hkv, D;
+  int32_t blocks;     /* blocks of a sequence in the contiguous form (block = sequence * blocks + j); 1: page pool */
+  int32_t tokens;     /* tokens a sequence has room for (64 in a page pool) */
+  int64_t num_blocks; /* all of them */
+} kvskip_write8_params;
+
+/* Writes tokens into the 8-bit cache.  The tokens of one block that stand next to each other in `slots`
+ * with ascending rows form a run; the values of a run get the block's scale
+ *     max(the block's scale so far, the smallest power of two s >= 2^-100 with max|x| <= qmax * s)
+ * (qmax 448 or 127; infinities are left out of the maximum and saturate, a NaN stays one in e4m3 and is
+ * 0 in int8).  A run that begins at row 0 starts the block afresh: what the block and its scale held
+ * before does not matter.  Otherwise, when the scale grows, the codes of the rows before the run are
+ * rounded to the new scale (exact for e4m3 short of its smallest values when the old scale is a power of
+ * two).  Rows behind the run stay as they are.  All runs of one call go to different blocks: a run that
+ * directly follows another one of the same block is skipped (status word 0x303), as is a slot
+ * outside the cache (0x302); runs of one block further apart in the list race for it. */
+int kvskip_launch_write8(const kvskip_write8_params* p, void* stream);
+
+/* Page and slot tables from request lengths, on the device.  Request b holds lens[b] tokens in the pages
+ * table[b, 0..ceil(lens[b]/64)) and is to get new_[b] more (negative counts as 0); free_pages
+ * [num_free] is a stack of the free pages, *n_free of them.  In the order of the requests, every request
+ * that fits (into max_pages pages, into the slot list, and into what the earlier ones left of the stack;
+ * one that needs no page always fits into the stack) is granted: its new blocks get pages from the top
+ * of the stack, written to the table, and its tokens their slot (page * 64 + row) and position.  Nothing
+ * of a refused request changes; its slots are -1.  Once one request has found too few pages, no later one
+ * gets a page.
+ * Slot lists: per_row = 0, packed: the tokens of request 0, 1, ... one after the other, n_tokens entries;
+ * per_row > 0: token i of request b at b * per_row + i (n_tokens = B * per_row).  Places without a token
+ * get -1.  lens_out and n_free_out may be lens and n_free themselves; the stack is not written. */
+typedef struct kvskip_pages_params {
+  const int32_t* lens;  /* [B] */
+  const int32_t* new_;  /* [B]; extend only */
+  const uint8_t* done;  /* [B]; release only */
+  int32_t* table;       /* [B,max_pages] */
+  int32_t* free_pages;  /* [num_free] */
+  const int32_t* n_free;
+  int32_t* lens_out;    /* [B] */
+  int32_t* n_free_out;
+  int64_t* slots;       /* [n_tokens]; extend only, as the next two */
+  int32_t* positions;   /* [n_tokens] */
+  uint8_t* granted;     /* [B] */
+  int64_t n_tokens;
+  int32_t per_row;
+  int32_t B, max_pages, num_free;
+} kvskip_pages_params;
+int kvskip_launch_extend_pages(const kvskip_pages_params* p, void* stream);
+/* The pages of every request with done[b] != 0 go back on top of the stack (in the order of requests and
+ * blocks; what would not fit into it is dropped) and its length becomes 0; the table is left as it is. */
+int kvskip_launch_release_pages(const kvskip_pages_params* p, void* stream);
+
 /* Process-wide options (no counterpart in the reference).
  *   "decode_path"  0 (default): tensor-core kernel for D = 128, exact-order kernel otherwise;
  *                  1: exact-order kernel everywhere -- scores, block statistics and outputs are
@@ -338,7 +454,8 @@ const char* kvskip_last_error(void);
 /* Reads (and clears) the current device's kernel status word after synchronising `stream`:
  * 0 if every bounded wait inside the kernels completed, otherwise the code of the first that
  * gave up (0x2xx / 0x4xx: a stage of a kernel's load ring; 0x300 / 0x301: a page table entry outside
- * the pool; 0x310: plan's hand-over inside a cluster; 0x500 + peer, 0x510 + peer: the exchange between
+ * the pool; 0x302 / 0x303: a slot outside the 8-bit cache, two runs of one block in a row; 0x6xx: a stage of
+ * the 8-bit attention's loads; 0x310: plan's hand-over inside a cluster; 0x500 + peer, 0x510 + peer: the exchange between
  * GPUs).  Host-blocking; meant for tests and post-mortems, not for the hot path.  When the word is
  * non-zero the call also waits for the whole device and clears the split counters a kernel that
  * gave up may have left behind: no launch of this library may be in flight on another host thread. */

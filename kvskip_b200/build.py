@@ -14,6 +14,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -35,8 +36,8 @@ LIB = out_dir() / "libkvskip_b200.so"
 EXT = out_dir() / "_kvskip_ext.so"
 
 NVCC_FLAGS = ["-O3", "--use_fast_math", "-lineinfo", "-std=c++17",
-              "-gencode", "arch=compute_100a,code=sm_100a",
-              "-shared", "-Xcompiler", "-fPIC"]
+              "-gencode", "arch=compute_100a,code=sm_100a", "-Xcompiler", "-fPIC"]
+UNITS = ("kvskip_b200", "cache8")        # translation units of the library: csrc/<name>.cu
 
 
 def _newer(target: Path, sources) -> bool:
@@ -57,11 +58,17 @@ def _run(cmd, verbose):
 
 
 def build_lib(force=False, verbose=False, ptxas_v=False) -> Path:
-    srcs = [CSRC / "kvskip_b200.cu", *CSRC.glob("*.cuh"), ROOT / "include" / "kvskip_b200.h"]
-    if force or _newer(LIB, srcs):
-        nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-        flags = list(NVCC_FLAGS) + (["-Xptxas", "-v"] if ptxas_v else [])
-        _run([nvcc, *flags, CSRC / "kvskip_b200.cu", "-o", LIB], verbose or ptxas_v)
+    """Compiles the translation units that are out of date, side by side, and links them."""
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    headers = [*CSRC.glob("*.cuh"), *CSRC.glob("*.h"), ROOT / "include" / "kvskip_b200.h"]
+    objs = {u: LIB.parent / f"{u}.o" for u in UNITS}
+    stale = [u for u in UNITS if force or _newer(objs[u], [CSRC / f"{u}.cu", *headers])]
+    if not force and not _newer(LIB, [*headers, *(CSRC / f"{u}.cu" for u in UNITS)]):
+        return LIB
+    flags = list(NVCC_FLAGS) + (["-Xptxas", "-v"] if ptxas_v else [])
+    with ThreadPoolExecutor() as pool:
+        list(pool.map(lambda u: _run([nvcc, *flags, "-c", CSRC / f"{u}.cu", "-o", objs[u]], verbose or ptxas_v), stale))
+    _run([nvcc, *NVCC_FLAGS, "-shared", *objs.values(), "-o", LIB], verbose or ptxas_v)
     return LIB
 
 

@@ -53,6 +53,33 @@ class UpdateParams(C.Structure):
                 ("level", _f32)]
 
 
+class Decode8Params(C.Structure):
+    _fields_ = [("q", _vp), ("q_sb", _i64), ("q_sh", _i64), ("k", _vp), ("v", _vp),
+                ("k_sb", _i64), ("k_sh", _i64), ("k_st", _i64), ("v_sb", _i64), ("v_sh", _i64), ("v_st", _i64),
+                ("k_scale", _vp), ("v_scale", _vp),
+                ("ks_sb", _i64), ("ks_sh", _i64), ("ks_st", _i64), ("vs_sb", _i64), ("vs_sh", _i64), ("vs_st", _i64),
+                ("q_f16", _i32), ("kind", _i32), ("B", _i32), ("Hq", _i32), ("Hkv", _i32), ("D", _i32), ("T", _i32),
+                ("scale_log2", _f32), ("lens", _vp), ("page_table", _vp), ("max_pages", _i32), ("num_pages", _i32),
+                ("block_idx", _vp), ("block_cnt", _vp), ("max_blocks", _i32), ("nb", _i32),
+                ("out", _vp), ("out_f32", _vp), ("lse", _vp), ("blk_max", _vp), ("blk_sum", _vp), ("work", _vp)]
+
+
+class Write8Params(C.Structure):
+    _fields_ = [("k_new", _vp), ("v_new", _vp), ("kn_so", _i64), ("kn_si", _i64), ("kn_sh", _i64),
+                ("vn_so", _i64), ("vn_si", _i64), ("vn_sh", _i64), ("n", _i64), ("inner", _i64), ("slots", _vp),
+                ("k", _vp), ("v", _vp), ("k_sb", _i64), ("k_sh", _i64), ("k_st", _i64),
+                ("v_sb", _i64), ("v_sh", _i64), ("v_st", _i64), ("k_scale", _vp), ("v_scale", _vp),
+                ("ks_sb", _i64), ("ks_sh", _i64), ("ks_st", _i64), ("vs_sb", _i64), ("vs_sh", _i64), ("vs_st", _i64),
+                ("x_f16", _i32), ("kind", _i32), ("Hkv", _i32), ("D", _i32), ("blocks", _i32), ("tokens", _i32),
+                ("num_blocks", _i64)]
+
+
+class PagesParams(C.Structure):
+    _fields_ = [("lens", _vp), ("new_", _vp), ("done", _vp), ("table", _vp), ("free_pages", _vp), ("n_free", _vp),
+                ("lens_out", _vp), ("n_free_out", _vp), ("slots", _vp), ("positions", _vp), ("granted", _vp),
+                ("n_tokens", _i64), ("per_row", _i32), ("B", _i32), ("max_pages", _i32), ("num_free", _i32)]
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 

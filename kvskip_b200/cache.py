@@ -13,6 +13,11 @@ a block straight from its page (the tensor map runs over the pool), so the plann
 and the page table together decide which pages a step touches; nothing is gathered.  The reference
 reads [B,Hkv,T,D] views only; its notes name this layout as the natural one for block skipping
 (docs/03-gate-digest.md:364).
+
+`PagedKV8` is a paged cache for a batch of requests of different lengths, in 8-bit codes with one scale
+per page and head, whose tables live on the device: handing out pages, writing tokens and
+reading them back through `kvskip.decode8` needs no host synchronisation, so a decode step can be captured
+once and replayed while the requests grow.
 """
 
 import math
@@ -163,3 +168,83 @@ class PagedKV:
 
     def get_seq_length(self) -> int:
         return self.n
+
+
+class PagedKV8:
+    """A pool of 64-token pages in 8-bit codes (float8_e4m3fn or int8) shared by up to B requests; row b of the
+    batch is request b, `lens[b]` tokens long (0: no request).
+
+        slots = cache.extend(new, per_row=S)     # pages for new[b] more tokens of every request
+        cache.write(k_new, v_new, slots)         # [B,Hkv,S,D] (or packed: [N,Hkv,D] with n_tokens=N)
+        out = cache.decode(q, scale)["out"]
+        cache.release(done)                      # pages of finished requests go back
+
+    Nothing here synchronises; a request that finds no page is refused (`granted`) and keeps its length.
+    `lens`, `table`, `free_pages` and `n_free` are device tensors that change in place."""
+
+    def __init__(self, num_pages: int, B: int, Hkv: int, D: int, max_tokens: int, device,
+                 dtype=torch.float8_e4m3fn):
+        if dtype not in (torch.float8_e4m3fn, torch.int8):
+            raise ValueError("PagedKV8: float8_e4m3fn or int8")
+        if D not in (64, 128):
+            raise ValueError("PagedKV8: head dim 64 or 128")
+        if min(num_pages, B, Hkv, max_tokens) < 1:
+            raise ValueError("PagedKV8: num_pages, B, Hkv and max_tokens are at least 1")
+        self.k = torch.zeros(num_pages, Hkv, BLOCK, D, dtype=torch.uint8, device=device).view(dtype)
+        self.v = torch.zeros(num_pages, Hkv, BLOCK, D, dtype=torch.uint8, device=device).view(dtype)
+        self.k_scale = torch.ones(num_pages, Hkv, dtype=torch.float32, device=device)
+        self.v_scale = torch.ones_like(self.k_scale)
+        self.B, self.max_pages = B, math.ceil(max_tokens / BLOCK)
+        self.lens = torch.zeros(B, dtype=torch.int32, device=device)
+        self.table = torch.full((B, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)   # page 0 on top
+        self.n_free = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+        self.granted = None
+        self.positions = None
+        self._ones = torch.ones(B, dtype=torch.int32, device=device)
+
+    def extend(self, new: torch.Tensor | None = None, *, n_tokens: int | None = None, per_row: int | None = None):
+        """Room for new[b] (int32 [B], default one) more tokens of every request; returns their slots (see
+        `kvskip.extend_pages`), `granted` and `positions` are kept on the object."""
+        if new is None:
+            new = self._ones
+        if n_tokens is None and per_row is None:
+            per_row = 1
+        r = K.extend_pages(self.lens, new, self.table, self.free_pages, self.n_free, n_tokens=n_tokens, per_row=per_row,
+                           lens_out=self.lens, n_free_out=self.n_free)
+        self.granted, self.positions = r["granted"], r["positions"]
+        return r["slots"]
+
+    def write(self, k_new: torch.Tensor, v_new: torch.Tensor, slots: torch.Tensor) -> None:
+        K.write8(k_new, v_new, slots, self.k, self.v, self.k_scale, self.v_scale)
+
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, new: torch.Tensor | None = None) -> None:
+        """One token per request, [B,Hkv,D] each; new (int32 [B] of 0 and 1) leaves rows out."""
+        slots = self.extend(new, per_row=1)
+        self.write(k_new.unsqueeze(2), v_new.unsqueeze(2), slots)
+
+    def release(self, done: torch.Tensor) -> None:
+        K.release_pages(done, self.lens, self.table, self.free_pages, self.n_free, lens_out=self.lens,
+                        n_free_out=self.n_free)
+
+    def decode(self, q, scale: float, plan=None, stats: bool = False, out_f32: bool = False,
+               max_len: int | None = None) -> dict:
+        return K.decode8(q, self.k, self.v, self.k_scale, self.v_scale, scale, lens=self.lens, page_table=self.table,
+                         max_len=max_len, plan=plan, stats=stats, out_f32=out_f32)
+
+    # hooks of kvskip_b200.graph.StepGraph: the lengths are on the device, a replayed step needs nothing here
+    def graph_scalars(self) -> tuple:
+        return ()
+
+    def note_replayed(self) -> None:
+        pass
+
+    def gather(self, b: int):
+        """fp32 copies [Hkv,n,D] of request b's keys and values (tests, debugging; reads the length back)."""
+        n = int(self.lens[b])
+        pages = self.table[b, :math.ceil(n / BLOCK)].long()
+        out = []
+        for codes, scale in ((self.k, self.k_scale), (self.v, self.v_scale)):
+            x = codes[pages].float() * scale[pages][:, :, None, None]
+            out.append(x.transpose(0, 1).reshape(x.shape[1], -1, x.shape[3])[:, :n])
+        return tuple(out)

@@ -1,0 +1,220 @@
+// C entry points of the 8-bit cache (see include/kvskip_b200.h): attention, write, page tables.
+// A translation unit of its own, compiled beside kvskip_b200.cu.
+#include "../../include/kvskip_b200.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "host.h"
+#include "common.cuh"
+#include "decode8.cuh"
+#include "write8.cuh"
+#include "pages.cuh"
+
+namespace {
+
+using kvb_host::fail;
+
+#define KVB_CUDA(expr)                                                                       \
+  do {                                                                                       \
+    cudaError_t e_ = (expr);                                                                 \
+    if (e_ != cudaSuccess) return fail(KVSKIP_E_CUDA, "%s: %s", #expr, cudaGetErrorString(e_)); \
+  } while (0)
+
+// Programmatic dependent launch: every kernel here waits for its predecessor before it touches global memory.
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = kvb_host::use_pdl() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+bool misaligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+
+// Map over [n,Hkv,rows,D] codes; one box is 64 rows of one head, swizzled over the row's D bytes.
+int make_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t st, int n, int Hkv, int rows, int D) {
+  const auto enc = kvb_host::encode_tiled();
+  if (!enc) return fail(KVSKIP_E_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  // a dim of size 1 may carry any stride (0 too): give the map a valid one
+  if (rows == 1 && st < D) st = D;
+  if (Hkv == 1 && sh <= 0) sh = static_cast<int64_t>(rows) * st;
+  if (n == 1 && sb <= 0) sb = static_cast<int64_t>(Hkv) * sh;
+  if (st <= 0 || sh <= 0 || sb <= 0) return fail(KVSKIP_E_ARG, "decode8: k / v strides must be positive");
+  const cuuint64_t gdim[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(Hkv),
+                              static_cast<cuuint64_t>(n)};
+  const cuuint64_t gstr[3] = {static_cast<cuuint64_t>(st), static_cast<cuuint64_t>(sh), static_cast<cuuint64_t>(sb)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(D), KVSKIP_TILE, 1, 1};
+  const cuuint32_t est[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), gdim, gstr, box, est,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(KVSKIP_E_CUDA, "cuTensorMapEncodeTiled failed (%d) for strides %lld/%lld/%lld dims %d/%d/%d/%d",
+                static_cast<int>(r), static_cast<long long>(sb), static_cast<long long>(sh), static_cast<long long>(st), n,
+                Hkv, rows, D);
+  return KVSKIP_OK;
+}
+
+// Fewest items (blocks of a head) of a CTA: below it fewer CTAs take part.
+constexpr int kMinItems = 4;
+
+template <int KIND, int D, int MODE>
+int launch_decode8(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cudaStream_t stream) {
+  using Cfg = kvb::D8Cfg<D, MODE>;
+  auto kernel = kvb::decode8_kernel<KIND, D, MODE>;
+  if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmem)) return rc;
+  const int64_t items = static_cast<int64_t>(p.B) * p.Hkv * (p.block_idx ? p.max_blocks : p.nb);
+  const int ctas = static_cast<int>(
+      std::max<int64_t>(1, std::min<int64_t>(std::min(kvb_host::num_sms(), kvb::D8_MAX_CTAS), (items + kMinItems - 1) / kMinItems)));
+  KVB_CUDA(launch(kernel, dim3(ctas), Cfg::kThreads, Cfg::kSmem, stream, p, maps, kMinItems));
+  if (ctas > 1) KVB_CUDA(launch(kvb::decode8_merge_kernel<D, MODE>, dim3(ctas), 256, 0, stream, p, ctas));
+  return KVSKIP_OK;
+}
+
+template <int KIND, int D>
+int by_group(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cudaStream_t s) {
+  const int G = p.Hq / p.Hkv;
+  if (G <= 4) return launch_decode8<KIND, D, 0>(p, maps, s);
+  if (G <= 8) return launch_decode8<KIND, D, 1>(p, maps, s);
+  return launch_decode8<KIND, D, 2>(p, maps, s);
+}
+
+template <int KIND, int D>
+int by_chunk(const kvskip_write8_params& p, cudaStream_t s) {
+  // The slots of a CTA: 64 when that still gives every SM work, else 8, so that the tokens of a decode step
+  // spread over the GPU.
+  if ((p.n + 63) / 64 * p.Hkv * 2 >= 2 * static_cast<int64_t>(kvb_host::num_sms()))
+    KVB_CUDA(launch(kvb::write8_kernel<KIND, D, 64>, dim3(static_cast<unsigned>((p.n + 63) / 64), p.Hkv, 2), kvb::W8_THREADS, 0, s, p));
+  else
+    KVB_CUDA(launch(kvb::write8_kernel<KIND, D, 8>, dim3(static_cast<unsigned>((p.n + 7) / 8), p.Hkv, 2), kvb::W8_THREADS, 0, s, p));
+  return KVSKIP_OK;
+}
+
+// CTAs for `n` table or slot entries
+int pages_grid(int64_t n) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kvb_host::num_sms(), n / 4096)));
+}
+
+int check_pages(const kvskip_pages_params* p, const char* who) {
+  if (!p) return fail(KVSKIP_E_ARG, "null parameter block");
+  if (!p->lens || !p->table || !p->free_pages || !p->n_free || !p->lens_out || !p->n_free_out)
+    return fail(KVSKIP_E_ARG, "%s: lens, table, free_pages, n_free, lens_out and n_free_out are required", who);
+  if (p->B < 1 || p->max_pages < 1 || p->num_free < 1) return fail(KVSKIP_E_ARG, "%s: B, max_pages, num_free >= 1", who);
+  if (p->max_pages > 2147483647 / KVSKIP_TILE) return fail(KVSKIP_E_LIMIT, "%s: more than 2^31 tokens per request", who);
+  return KVSKIP_OK;
+}
+
+}  // namespace
+
+namespace kvb_host {
+int cache8_status(unsigned int* status) {
+  KVB_CUDA(cudaMemcpyFromSymbol(status, kvb::g_status, sizeof(unsigned int)));
+  if (*status) {
+    const unsigned int zero = 0;
+    KVB_CUDA(cudaDeviceSynchronize());
+    KVB_CUDA(cudaMemcpyToSymbol(kvb::g_status, &zero, sizeof(zero)));
+  }
+  return KVSKIP_OK;
+}
+}  // namespace kvb_host
+
+extern "C" {
+
+int64_t kvskip_decode8_work_bytes(int G, int D) {
+  if (G < 1 || G > 16 || (D != 64 && D != 128)) return 0;
+  const int64_t cols = G <= 4 ? 4 : G <= 8 ? 8 : 16;
+  return kvb::D8_MAX_CTAS * (2 * cols * (D + 2) * static_cast<int64_t>(sizeof(float)) + 2 * static_cast<int64_t>(sizeof(int)));
+}
+
+int kvskip_launch_decode8(const kvskip_decode8_params* p, void* stream) {
+  if (!p) return fail(KVSKIP_E_ARG, "null parameter block");
+  if (p->D != 64 && p->D != 128) return fail(KVSKIP_E_ARG, "decode8: head dim 64 or 128");
+  if (p->kind != KVSKIP_KIND_E4M3 && p->kind != KVSKIP_KIND_INT8) return fail(KVSKIP_E_ARG, "decode8: kind 0 (e4m3) or 1 (int8)");
+  if (p->B < 1 || p->Hkv < 1 || p->T < 1 || p->Hq < 1 || p->Hq % p->Hkv) return fail(KVSKIP_E_ARG, "decode8: bad B / Hq / Hkv / T");
+  if (p->Hq / p->Hkv > 16) return fail(KVSKIP_E_ARG, "decode8: at most 16 query heads per KV head");
+  if (!p->q || !p->k || !p->v || !p->k_scale || !p->v_scale || !p->out || !p->lse || !p->work)
+    return fail(KVSKIP_E_ARG, "decode8: q, k, v, k_scale, v_scale, out, lse and work are required");
+  if (p->nb != (p->T - 1) / KVSKIP_TILE + 1) return fail(KVSKIP_E_ARG, "decode8: nb must be ceil(T / 64)");
+  if ((p->block_idx == nullptr) != (p->block_cnt == nullptr) || (p->block_idx && p->max_blocks < 1))
+    return fail(KVSKIP_E_ARG, "decode8: block_idx, block_cnt and max_blocks go together");
+  if ((p->blk_max == nullptr) != (p->blk_sum == nullptr)) return fail(KVSKIP_E_ARG, "decode8: blk_max and blk_sum go together");
+  if (p->page_table && (p->num_pages < 1 || p->max_pages < p->nb))
+    return fail(KVSKIP_E_ARG, "paged cache: the page table needs an entry for every block of the sequence");
+  if (p->page_table && !p->lens) return fail(KVSKIP_E_ARG, "decode8: a paged cache needs lens");
+  if (misaligned(p->q, 8) || p->q_sb % 4 || p->q_sh % 4) return fail(KVSKIP_E_ARG, "decode8: q rows must be 8-byte aligned");
+  if (misaligned(p->out, 4) || misaligned(p->out_f32, 8) || misaligned(p->work, 16))
+    return fail(KVSKIP_E_ARG, "decode8: misaligned out / out_f32 / work");
+  if (misaligned(p->k, 16) || misaligned(p->v, 16) || (p->k_sb | p->k_sh | p->k_st | p->v_sb | p->v_sh | p->v_st) % 16)
+    return fail(KVSKIP_E_ARG, "decode8: k / v must be 16-byte aligned, with strides that are multiples of 16");
+  if (static_cast<int64_t>(p->B) * p->Hkv * (p->block_idx ? std::max(p->max_blocks, p->nb) : p->nb) > 2147483647LL ||
+      static_cast<int64_t>(p->B) * p->Hq > 2147483647LL)
+    return fail(KVSKIP_E_LIMIT, "decode8: more than 2^31 blocks of heads in a call");
+  kvb::D8Maps maps;
+  const int n = p->page_table ? p->num_pages : p->B, rows = p->page_table ? KVSKIP_TILE : p->T;
+  if (int rc = make_map(&maps.k, p->k, p->k_sb, p->k_sh, p->k_st, n, p->Hkv, rows, p->D)) return rc;
+  if (int rc = make_map(&maps.v, p->v, p->v_sb, p->v_sh, p->v_st, n, p->Hkv, rows, p->D)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->kind == KVSKIP_KIND_E4M3)
+    return p->D == 128 ? by_group<KVSKIP_KIND_E4M3, 128>(*p, maps, s) : by_group<KVSKIP_KIND_E4M3, 64>(*p, maps, s);
+  return p->D == 128 ? by_group<KVSKIP_KIND_INT8, 128>(*p, maps, s) : by_group<KVSKIP_KIND_INT8, 64>(*p, maps, s);
+}
+
+int kvskip_launch_write8(const kvskip_write8_params* p, void* stream) {
+  if (!p) return fail(KVSKIP_E_ARG, "null parameter block");
+  if (p->D != 64 && p->D != 128) return fail(KVSKIP_E_ARG, "write8: head dim 64 or 128");
+  if (p->kind != KVSKIP_KIND_E4M3 && p->kind != KVSKIP_KIND_INT8) return fail(KVSKIP_E_ARG, "write8: kind 0 (e4m3) or 1 (int8)");
+  if (p->n < 0 || p->inner < 1 || p->Hkv < 1 || p->blocks < 1 || p->tokens < 1 || p->num_blocks < 1)
+    return fail(KVSKIP_E_ARG, "write8: bad n / inner / Hkv / blocks / tokens / num_blocks");
+  if (p->n == 0) return KVSKIP_OK;
+  if (!p->k_new || !p->v_new || !p->slots || !p->k || !p->v || !p->k_scale || !p->v_scale)
+    return fail(KVSKIP_E_ARG, "write8: k_new, v_new, slots, k, v, k_scale and v_scale are required");
+  if (misaligned(p->k_new, 16) || misaligned(p->v_new, 16) ||
+      (p->kn_so | p->kn_si | p->kn_sh | p->vn_so | p->vn_si | p->vn_sh) % 8)
+    return fail(KVSKIP_E_ARG, "write8: rows of k_new and v_new must be 16-byte aligned");
+  if (misaligned(p->k, 8) || misaligned(p->v, 8) || (p->k_sb | p->k_sh | p->k_st | p->v_sb | p->v_sh | p->v_st) % 8)
+    return fail(KVSKIP_E_ARG, "write8: rows of k and v must be 8-byte aligned");
+  if (p->Hkv > 65535 || (p->n + 7) / 8 > 2147483647LL) return fail(KVSKIP_E_LIMIT, "write8: grid limits exceeded");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->kind == KVSKIP_KIND_E4M3)
+    return p->D == 128 ? by_chunk<KVSKIP_KIND_E4M3, 128>(*p, s) : by_chunk<KVSKIP_KIND_E4M3, 64>(*p, s);
+  return p->D == 128 ? by_chunk<KVSKIP_KIND_INT8, 128>(*p, s) : by_chunk<KVSKIP_KIND_INT8, 64>(*p, s);
+}
+
+int kvskip_launch_extend_pages(const kvskip_pages_params* p, void* stream) {
+  if (int rc = check_pages(p, "extend_pages")) return rc;
+  if (!p->new_ || !p->granted || (p->n_tokens > 0 && (!p->slots || !p->positions)))
+    return fail(KVSKIP_E_ARG, "extend_pages: new, granted, slots and positions are required");
+  if (p->n_tokens < 0 || p->per_row < 0 || (p->per_row > 0 && p->n_tokens != static_cast<int64_t>(p->per_row) * p->B))
+    return fail(KVSKIP_E_ARG, "extend_pages: n_tokens >= 0, and B * per_row of them in a padded list");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int grid = pages_grid(p->n_tokens);
+  const bool in_place = p->lens_out == p->lens || p->n_free_out == p->n_free;
+  const int one = grid == 1 || !in_place;       // several CTAs read lens and n_free: they change in a launch behind
+  KVB_CUDA(launch(kvb::extend_pages_kernel, dim3(grid), kvb::PG_THREADS, 0, s, *p, 1, one));
+  if (!one) KVB_CUDA(launch(kvb::extend_pages_kernel, dim3(1), kvb::PG_THREADS, 0, s, *p, 0, 1));
+  return KVSKIP_OK;
+}
+
+int kvskip_launch_release_pages(const kvskip_pages_params* p, void* stream) {
+  if (int rc = check_pages(p, "release_pages")) return rc;
+  if (!p->done) return fail(KVSKIP_E_ARG, "release_pages: done is required");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int grid = pages_grid(static_cast<int64_t>(p->B) * p->max_pages / 8);
+  const bool in_place = p->lens_out == p->lens || p->n_free_out == p->n_free;
+  const int one = grid == 1 || !in_place;
+  KVB_CUDA(launch(kvb::release_pages_kernel, dim3(grid), kvb::PG_THREADS, 0, s, *p, 1, one));
+  if (!one) KVB_CUDA(launch(kvb::release_pages_kernel, dim3(1), kvb::PG_THREADS, 0, s, *p, 0, 1));
+  return KVSKIP_OK;
+}
+
+}  // extern "C"

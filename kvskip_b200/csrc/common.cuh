@@ -20,9 +20,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 // limit, so this is seconds of wall time, far beyond any legitimate wait for an HBM load.
 constexpr uint32_t SPIN_LIMIT = 1u << 22;
 
-// Device status word of the library (one per loaded module / device): 0 = fine; otherwise the
+// Device status word (one per translation unit / device): 0 = fine; otherwise the
 // code of the first wait that timed out.  Read back by kvskip_device_status().
-static __device__ unsigned int g_status = 0;   // the library is one translation unit: one copy per device
+static __device__ unsigned int g_status = 0;   // one copy per device and translation unit
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -1,5 +1,5 @@
 // libkvskip_b200: C ABI over the sm_100a kernels (see include/kvskip_b200.h).
-// Single translation unit: the kernels live in the .cuh files included below.
+// The kernels live in the .cuh files included below; those of the 8-bit cache are in cache8.cu.
 #include "../../include/kvskip_b200.h"
 
 #include <cuda.h>
@@ -15,6 +15,7 @@
 #include <string>
 #include <utility>
 
+#include "host.h"
 #include "common.cuh"
 #include "decode_exact.cuh"
 #include "decode_tc.cuh"
@@ -416,6 +417,27 @@ int launch_pv_t(const kvskip_params& p, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// what cache8.cu uses of the helpers above
+namespace kvb_host {
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  t_error = buf;
+  return code;
+}
+int ensure_smem(const void* func, int bytes) { return ::ensure_smem(func, bytes); }
+bool use_pdl() { return g_use_pdl.load(std::memory_order_relaxed) != 0; }
+int num_sms() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+EncodeTiledFn encode_tiled() { return encode_tiled_fn(); }
+}  // namespace kvb_host
 
 extern "C" {
 
@@ -1004,6 +1026,9 @@ int kvskip_device_status(void* stream, unsigned int* status) {
     KVB_CUDA(cudaGetSymbolAddress(&ptr, g_split_done));
     KVB_CUDA(cudaMemset(ptr, 0, sizeof(int) * kMergeRegion * kMergeRegions));
   }
+  unsigned int st8 = 0;                       // the kernels of cache8.cu have a word of their own
+  if (int rc = kvb_host::cache8_status(&st8)) return rc;
+  if (!*status) *status = st8;
   return KVSKIP_OK;
 }
 

@@ -704,6 +704,251 @@ void advance(at::Tensor& t_dev, int64_t delta) {
   raise_on(kvskip_launch_advance(t_dev.data_ptr<int32_t>(), static_cast<int>(delta), cur_stream()));
 }
 
+// ---- 8-bit cache ---------------------------------------------------------------------------------
+int kind_of(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && (t.scalar_type() == at::kFloat8_e4m3fn || t.scalar_type() == at::kChar), name,
+              " must be a CUDA float8_e4m3fn or int8 tensor");
+  TORCH_CHECK(t.dim() == 4 && t.stride(3) == 1, name, " must be [pages, Hkv, 64, D] or [B, Hkv, T, D] with a contiguous last dim");
+  TORCH_CHECK(t.stride(2) % 16 == 0 && t.stride(1) % 16 == 0 && t.stride(0) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " rows must be 16-byte aligned");
+  return t.scalar_type() == at::kChar ? KVSKIP_KIND_INT8 : KVSKIP_KIND_E4M3;
+}
+void need_x16(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf), name,
+              " must be a CUDA bf16 or fp16 tensor");
+}
+const int32_t* i32(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kInt && t.is_contiguous(), name, ": contiguous CUDA int32");
+  return t.data_ptr<int32_t>();
+}
+void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> others) {
+  for (const at::Tensor* t : others) TORCH_CHECK(t->device() == a.device(), "all tensors must be on one device");
+}
+// k, v and their scales: paged (scales [pages, Hkv]) or contiguous (scales [B, Hkv, >= nb])
+int check_cache8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs, bool paged) {
+  const int kind = kind_of(k, "k");
+  TORCH_CHECK(kind_of(v, "v") == kind && v.sizes() == k.sizes(), "k and v must share type and shape");
+  TORCH_CHECK(ks.is_cuda() && vs.is_cuda() && ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat,
+              "k_scale, v_scale: CUDA fp32");
+  if (paged) {
+    TORCH_CHECK(k.size(2) == KVSKIP_TILE, "paged cache: pools are [pages, Hkv, 64, D]");
+    TORCH_CHECK(ks.dim() == 2 && ks.size(0) == k.size(0) && ks.size(1) == k.size(1) && vs.sizes() == ks.sizes(),
+                "paged cache: scales are [pages, Hkv]");
+  } else {
+    const int64_t nb = (k.size(2) + KVSKIP_TILE - 1) / KVSKIP_TILE;
+    for (const at::Tensor* t : {&ks, &vs})
+      TORCH_CHECK(t->dim() == 3 && t->size(0) == k.size(0) && t->size(1) == k.size(1) && t->size(2) >= nb,
+                  "contiguous cache: scales are [B, Hkv, ceil(T / 64)]");
+  }
+  same_device(k, {&v, &ks, &vs});
+  return kind;
+}
+uint8_t* u8(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+// [out of q's type [B,Hq,D], lse [B,Hq], blk_max, blk_sum ([B,Hq,nb] or undefined), out_f32 or undefined]
+std::vector<at::Tensor> decode8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_scale,
+                                const at::Tensor& v_scale, double scale, const c10::optional<at::Tensor>& lens,
+                                const c10::optional<at::Tensor>& page_table, int64_t max_len,
+                                const c10::optional<at::Tensor>& block_idx, const c10::optional<at::Tensor>& block_cnt,
+                                bool stats, bool want_f32) {
+  need_x16(q, "q");
+  TORCH_CHECK(q.dim() == 3 && q.stride(2) == 1 && q.stride(1) % 4 == 0 && q.stride(0) % 4 == 0 &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0, "q must be [B, Hq, D] with 8-byte aligned rows");
+  const bool paged = page_table.has_value();
+  const int kind = check_cache8(k, v, k_scale, v_scale, paged);
+  same_device(q, {&k});
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
+  TORCH_CHECK(k.size(3) == D && (paged || k.size(0) == B), "shape mismatch between q, k, v");
+  TORCH_CHECK(D == 64 || D == 128, "decode8: head dim 64 or 128");
+  TORCH_CHECK(Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= 16, "Hq must be 1 to 16 times Hkv");
+  TORCH_CHECK(B >= 1, "decode8: an empty batch");
+  kvskip_decode8_params p{};
+  int64_t T = k.size(2);
+  if (paged) {
+    TORCH_CHECK(lens.has_value(), "a paged cache needs lens");
+    p.page_table = i32(*page_table, "page_table");
+    TORCH_CHECK(page_table->dim() == 2 && page_table->size(0) == B && page_table->size(1) >= 1, "page_table: [B, max_pages]");
+    T = page_table->size(1) * KVSKIP_TILE;
+    p.max_pages = static_cast<int32_t>(page_table->size(1));
+    p.num_pages = static_cast<int32_t>(k.size(0));
+    same_device(q, {&*page_table});
+  }
+  if (max_len > 0) {
+    TORCH_CHECK(max_len <= T, "max_len is beyond the cache");
+    T = max_len;
+  }
+  TORCH_CHECK(T >= 1 && T <= std::numeric_limits<int32_t>::max() - KVSKIP_TILE, "decode8: bad length");
+  const int64_t nb = (T + KVSKIP_TILE - 1) / KVSKIP_TILE;
+  if (lens.has_value()) {
+    p.lens = i32(*lens, "lens");
+    TORCH_CHECK(lens->numel() == B, "lens: [B]");
+    same_device(q, {&*lens});
+  }
+  TORCH_CHECK(block_idx.has_value() == block_cnt.has_value(), "block_cnt is required with block_idx");
+  if (block_idx.has_value()) {
+    p.block_idx = i32(*block_idx, "block_idx");
+    p.block_cnt = i32(*block_cnt, "block_cnt");
+    TORCH_CHECK(block_idx->dim() == 3 && block_idx->size(0) == B && block_idx->size(1) == Hkv && block_idx->size(2) >= 1,
+                "block_idx must be contiguous int32 [B, Hkv, max_blocks]");
+    TORCH_CHECK(block_cnt->numel() == B * Hkv, "block_cnt must be contiguous int32 [B, Hkv]");
+    p.max_blocks = static_cast<int32_t>(block_idx->size(2));
+    same_device(q, {&*block_idx, &*block_cnt});
+  }
+  const auto f32 = q.options().dtype(at::kFloat);
+  at::Tensor out = at::empty({B, Hq, D}, q.options()), lse = at::empty({B, Hq}, f32), out32, bmax, bsum;
+  if (want_f32) out32 = at::empty({B, Hq, D}, f32);
+  if (stats) {
+    bmax = at::empty({B, Hq, nb}, f32);
+    bsum = at::empty({B, Hq, nb}, f32);
+    p.blk_max = bmax.data_ptr<float>();
+    p.blk_sum = bsum.data_ptr<float>();
+  }
+  const int G = static_cast<int>(Hq / Hkv);
+  at::Tensor work = at::empty({kvskip_decode8_work_bytes(G, static_cast<int>(D))}, q.options().dtype(at::kByte));
+  p.q = u16(q);
+  p.q_sb = q.stride(0); p.q_sh = q.stride(1);
+  p.k = u8(k); p.v = u8(v);
+  p.k_sb = k.stride(0); p.k_sh = k.stride(1); p.k_st = k.stride(2);
+  p.v_sb = v.stride(0); p.v_sh = v.stride(1); p.v_st = v.stride(2);
+  p.k_scale = k_scale.data_ptr<float>(); p.v_scale = v_scale.data_ptr<float>();
+  p.ks_sb = k_scale.stride(0); p.ks_sh = k_scale.stride(1); p.ks_st = paged ? 0 : k_scale.stride(2);
+  p.vs_sb = v_scale.stride(0); p.vs_sh = v_scale.stride(1); p.vs_st = paged ? 0 : v_scale.stride(2);
+  p.q_f16 = q.scalar_type() == at::kHalf;
+  p.kind = kind;
+  p.B = static_cast<int32_t>(B); p.Hq = static_cast<int32_t>(Hq); p.Hkv = static_cast<int32_t>(Hkv);
+  p.D = static_cast<int32_t>(D);
+  p.T = static_cast<int32_t>(T);
+  p.nb = static_cast<int32_t>(nb);
+  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.out = u16m(out);
+  if (want_f32) p.out_f32 = out32.data_ptr<float>();
+  p.lse = lse.data_ptr<float>();
+  p.work = work.data_ptr();
+  raise_on(kvskip_launch_decode8(&p, cur_stream()));
+  return {out, lse, bmax, bsum, out32};
+}
+
+// k_new, v_new [N,Hkv,D] with slots [N], or [B,Hkv,S,D] with slots [B,S], into k, v, k_scale, v_scale
+void write8(const at::Tensor& k_new, const at::Tensor& v_new, const at::Tensor& slots, at::Tensor& k, at::Tensor& v,
+            at::Tensor& k_scale, at::Tensor& v_scale) {
+  need_x16(k_new, "k_new");
+  const bool paged = k_scale.dim() == 2;
+  const int kind = check_cache8(k, v, k_scale, v_scale, paged);
+  const int64_t Hkv = k.size(1), D = k.size(3);
+  TORCH_CHECK(D == 64 || D == 128, "write8: head dim 64 or 128");
+  TORCH_CHECK(v_new.scalar_type() == k_new.scalar_type() && v_new.sizes() == k_new.sizes(), "k_new and v_new must share type and shape");
+  TORCH_CHECK(slots.is_cuda() && slots.scalar_type() == at::kLong && slots.is_contiguous(), "slots: contiguous CUDA int64");
+  const bool flat = k_new.dim() == 3;
+  TORCH_CHECK((flat && k_new.size(1) == Hkv && k_new.size(2) == D && slots.dim() == 1 && slots.size(0) == k_new.size(0)) ||
+                  (k_new.dim() == 4 && k_new.size(1) == Hkv && k_new.size(3) == D && slots.dim() == 2 &&
+                   slots.size(0) == k_new.size(0) && slots.size(1) == k_new.size(2)),
+              "k_new, v_new: [N, Hkv, D] with slots [N], or [B, Hkv, S, D] with slots [B, S]");
+  same_device(k, {&k_new, &v_new, &slots});
+  const c10::cuda::CUDAGuard guard(k.device());
+  if (slots.numel() == 0) return;
+  kvskip_write8_params p{};
+  p.n = slots.numel();
+  p.inner = flat ? p.n : slots.size(1);
+  const auto strides = [&](const at::Tensor& t, const char* name, int64_t& so, int64_t& si, int64_t& sh) {
+    const int64_t last = t.dim() - 1;
+    TORCH_CHECK(t.stride(last) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && (flat || t.stride(2) % 8 == 0) &&
+                    reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " rows must be 16-byte aligned");
+    so = flat ? 0 : t.stride(0);
+    si = flat ? t.stride(0) : t.stride(2);
+    sh = t.stride(1);
+  };
+  strides(k_new, "k_new", p.kn_so, p.kn_si, p.kn_sh);
+  strides(v_new, "v_new", p.vn_so, p.vn_si, p.vn_sh);
+  p.k_new = u16(k_new); p.v_new = u16(v_new);
+  p.slots = slots.data_ptr<int64_t>();
+  p.k = u8(k); p.v = u8(v);
+  p.k_sb = k.stride(0); p.k_sh = k.stride(1); p.k_st = k.stride(2);
+  p.v_sb = v.stride(0); p.v_sh = v.stride(1); p.v_st = v.stride(2);
+  p.k_scale = k_scale.data_ptr<float>(); p.v_scale = v_scale.data_ptr<float>();
+  p.ks_sb = k_scale.stride(0); p.ks_sh = k_scale.stride(1); p.ks_st = paged ? 0 : k_scale.stride(2);
+  p.vs_sb = v_scale.stride(0); p.vs_sh = v_scale.stride(1); p.vs_st = paged ? 0 : v_scale.stride(2);
+  p.x_f16 = k_new.scalar_type() == at::kHalf;
+  p.kind = kind;
+  p.Hkv = static_cast<int32_t>(Hkv); p.D = static_cast<int32_t>(D);
+  p.tokens = static_cast<int32_t>(k.size(2));
+  p.blocks = paged ? 1 : static_cast<int32_t>((k.size(2) + KVSKIP_TILE - 1) / KVSKIP_TILE);
+  p.num_blocks = k.size(0) * p.blocks;
+  raise_on(kvskip_launch_write8(&p, cur_stream()));
+}
+
+void fill_pages(kvskip_pages_params& p, const at::Tensor& lens, const at::Tensor& page_table, const at::Tensor& free_pages,
+                const at::Tensor& n_free, const c10::optional<at::Tensor>& lens_out,
+                const c10::optional<at::Tensor>& n_free_out, at::Tensor& lo, at::Tensor& fo) {
+  p.lens = i32(lens, "lens");
+  i32(page_table, "page_table");
+  i32(free_pages, "free_pages");
+  p.n_free = i32(n_free, "n_free");
+  TORCH_CHECK(lens.dim() == 1 && lens.size(0) >= 1 && page_table.dim() == 2 && page_table.size(0) == lens.size(0) &&
+                  page_table.size(1) >= 1, "lens: [B], page_table: [B, max_pages]");
+  TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) >= 1 && n_free.numel() == 1, "free_pages: [pages], n_free: one element");
+  same_device(lens, {&page_table, &free_pages, &n_free});
+  lo = lens_out.has_value() ? *lens_out : at::empty_like(lens);
+  fo = n_free_out.has_value() ? *n_free_out : at::empty_like(n_free);
+  p.lens_out = const_cast<int32_t*>(i32(lo, "lens_out"));
+  p.n_free_out = const_cast<int32_t*>(i32(fo, "n_free_out"));
+  TORCH_CHECK(lo.numel() == lens.numel() && fo.numel() == 1, "lens_out: [B], n_free_out: one element");
+  same_device(lens, {&lo, &fo});
+  p.table = page_table.data_ptr<int32_t>();
+  p.free_pages = free_pages.data_ptr<int32_t>();
+  p.B = static_cast<int32_t>(lens.size(0));
+  p.max_pages = static_cast<int32_t>(page_table.size(1));
+  p.num_free = static_cast<int32_t>(free_pages.size(0));
+}
+
+// [slots int64, positions int32 ([n_tokens] or [B, per_row]), granted bool [B], lens_out, n_free_out]
+std::vector<at::Tensor> extend_pages(const at::Tensor& lens, const at::Tensor& new_, const at::Tensor& page_table,
+                                     const at::Tensor& free_pages, const at::Tensor& n_free, int64_t n_tokens,
+                                     int64_t per_row, const c10::optional<at::Tensor>& lens_out,
+                                     const c10::optional<at::Tensor>& n_free_out) {
+  TORCH_CHECK(lens.is_cuda(), "lens: contiguous CUDA int32");
+  const c10::cuda::CUDAGuard guard(lens.device());
+  kvskip_pages_params p{};
+  at::Tensor lo, fo;
+  fill_pages(p, lens, page_table, free_pages, n_free, lens_out, n_free_out, lo, fo);
+  p.new_ = i32(new_, "new");
+  TORCH_CHECK(new_.numel() == lens.numel(), "new: [B]");
+  same_device(lens, {&new_});
+  const int64_t B = lens.size(0);
+  TORCH_CHECK(per_row >= 0 && n_tokens >= 0 && (per_row == 0 || per_row <= std::numeric_limits<int32_t>::max()),
+              "extend_pages: n_tokens or per_row");
+  const int64_t n = per_row ? B * per_row : n_tokens;
+  const std::vector<int64_t> shape = per_row ? std::vector<int64_t>{B, per_row} : std::vector<int64_t>{n};
+  at::Tensor slots = at::empty(shape, lens.options().dtype(at::kLong));
+  at::Tensor positions = at::empty(shape, lens.options());
+  at::Tensor granted = at::empty({B}, lens.options().dtype(at::kBool));
+  p.slots = slots.data_ptr<int64_t>();
+  p.positions = positions.data_ptr<int32_t>();
+  p.granted = static_cast<uint8_t*>(granted.data_ptr());
+  p.n_tokens = n;
+  p.per_row = static_cast<int32_t>(per_row);
+  raise_on(kvskip_launch_extend_pages(&p, cur_stream()));
+  return {slots, positions, granted, lo, fo};
+}
+
+// [lens_out, n_free_out]
+std::vector<at::Tensor> release_pages(const at::Tensor& done, const at::Tensor& lens, const at::Tensor& page_table,
+                                      at::Tensor& free_pages, const at::Tensor& n_free,
+                                      const c10::optional<at::Tensor>& lens_out,
+                                      const c10::optional<at::Tensor>& n_free_out) {
+  TORCH_CHECK(lens.is_cuda(), "lens: contiguous CUDA int32");
+  TORCH_CHECK(done.is_cuda() && (done.scalar_type() == at::kBool || done.scalar_type() == at::kByte) && done.is_contiguous() &&
+                  done.numel() == lens.numel(), "done: contiguous CUDA bool or uint8 [B]");
+  const c10::cuda::CUDAGuard guard(lens.device());
+  kvskip_pages_params p{};
+  at::Tensor lo, fo;
+  fill_pages(p, lens, page_table, free_pages, n_free, lens_out, n_free_out, lo, fo);
+  same_device(lens, {&done});
+  p.done = u8(done);
+  raise_on(kvskip_launch_release_pages(&p, cur_stream()));
+  return {lo, fo};
+}
+
 void set_option(const std::string& name, int64_t value) {
   raise_on(kvskip_set_option(name.c_str(), static_cast<int>(value)));
 }
@@ -781,6 +1026,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("t_dev") = py::none(), py::arg("T_bound") = 0);
   m.def("advance", &advance, "device-resident sequence length += delta, in stream order", py::arg("t_dev"),
         py::arg("delta") = 1);
+  m.def("decode8", &decode8, "attention of one token per sequence over a cache of 8-bit codes with block scales",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_scale"), py::arg("v_scale"), py::arg("scale"),
+        py::arg("lens") = py::none(), py::arg("page_table") = py::none(), py::arg("max_len") = 0,
+        py::arg("block_idx") = py::none(), py::arg("block_cnt") = py::none(), py::arg("stats") = false,
+        py::arg("want_f32") = false);
+  m.def("write8", &write8, "new tokens into a cache of 8-bit codes with block scales", py::arg("k_new"), py::arg("v_new"),
+        py::arg("slots"), py::arg("k"), py::arg("v"), py::arg("k_scale"), py::arg("v_scale"));
+  m.def("extend_pages", &extend_pages, "pages and slots for the new tokens of every request", py::arg("lens"),
+        py::arg("new"), py::arg("page_table"), py::arg("free_pages"), py::arg("n_free"), py::arg("n_tokens") = 0,
+        py::arg("per_row") = 0, py::arg("lens_out") = py::none(), py::arg("n_free_out") = py::none());
+  m.def("release_pages", &release_pages, "pages of finished requests back to the free stack", py::arg("done"),
+        py::arg("lens"), py::arg("page_table"), py::arg("free_pages"), py::arg("n_free"),
+        py::arg("lens_out") = py::none(), py::arg("n_free_out") = py::none());
   m.def("set_option", &set_option, "process-wide option, e.g. (\"decode_path\", 1) for the exact-order kernels",
         py::arg("name"), py::arg("value"));
   m.def("get_option", &get_option, py::arg("name"));

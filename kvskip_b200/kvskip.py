@@ -10,6 +10,8 @@ to this module through the `kernels/` package at the repository root).
     decode(q, k, v, scale, stats=True)                      + per-block max and sum-exp
     decode(q, k, v, scale, stats=True, load_v=False)        statistics only: K is read, V is not
     vskip_one_pass / vskip_two_pass / pv                    V-skip variants
+    decode8 / write8 / extend_pages / release_pages         a cache of 8-bit codes with block scales, one
+                                                            length per sequence, page tables on the device
 
 q is [B, Hq, D] or [B, Hq, 1, D]; k, v are [B, Hkv, T, D] views with any batch/head/token strides
 and D contiguous.  Blocks are 64 tokens counted from position 0.
@@ -332,3 +334,75 @@ def vskip_one_pass(q, k, v, scale: float, tau: float = 1e-4, local: int = 2, num
         if sync:
             res["kept_frac"] = (cnt.sum() / (B * Hkv * nb)).item()
     return res
+
+
+def decode8(q, k, v, k_scale, v_scale, scale: float, *, lens: torch.Tensor | None = None,
+            page_table: torch.Tensor | None = None, max_len: int | None = None, plan: Plan | None = None,
+            stats: bool = False, out_f32: bool = False) -> dict:
+    """`decode` over a cache of 8-bit codes with one scale per 64-token block and KV head (value = code *
+    scale), with one length per sequence.  Not in the reference.
+
+    q bf16 or fp16 [B,Hq,D] or [B,Hq,1,D], Hq = 1 to 16 times Hkv, D 64 or 128.  k, v are float8_e4m3fn or
+    int8: page pools [pages,Hkv,64,D] with page_table int32 [B,max_pages] and k_scale, v_scale fp32
+    [pages,Hkv] (`kvskip_b200.cache.PagedKV8`), or contiguous views [B,Hkv,T,D] with scales
+    [B,Hkv,ceil(T/64)].  lens int32 [B] is read on the device (clamped to what the cache holds, or to max_len,
+    which bounds the launch and the statistics rows); without it every sequence of a contiguous
+    cache has T tokens.  A sequence of length 0 gives out = 0, lse = -inf; rows behind a length may hold anything.
+    plan: only the listed blocks are read (`make_plan`; its length is not read back).
+    Returns dict(out of q's type, lse fp32 [B,Hq][, blk_max, blk_sum fp32 [B,Hq,nb]][, out_f32])."""
+    if q.dim() == 4:
+        q = q.squeeze(2)
+    bi, bc = (None, None) if plan is None else (plan.block_idx, plan.block_cnt)
+    out, lse, bmax, bsum, o32 = ext().decode8(q, k, v, k_scale, v_scale, scale, lens, page_table, max_len or 0, bi, bc,
+                                              stats, out_f32)
+    _auto_check("decode8")
+    res = {"out": out, "lse": lse}
+    if stats:
+        res["blk_max"], res["blk_sum"] = bmax, bsum
+    if out_f32:
+        res["out_f32"] = o32
+    return res
+
+
+def write8(k_new, v_new, slots, k, v, k_scale, v_scale) -> None:
+    """New tokens into an 8-bit cache (both forms of `decode8`), in place.  Not in the reference.
+
+    k_new, v_new bf16 or fp16 [N,Hkv,D] with slots int64 [N], or [B,Hkv,S,D] with slots [B,S].  A slot is page *
+    64 + row, or in a contiguous cache (sequence * ceil(T/64) + block) * 64 + row; a negative one skips its token
+    (padding).  Tokens of one block stand next to each other with ascending rows, as `extend_pages` lists
+    them.  The scale of a block is the smallest power of two that covers its values so far; when a token
+    makes it grow, the codes already there are rounded to the new scale.  A token in row 0 starts its block
+    afresh, whatever page and scale held before.  Infinities saturate; a NaN stays one in e4m3 and is 0 in int8.
+    A slot outside the cache is skipped and sets the status word (`check_status`)."""
+    ext().write8(k_new, v_new, slots, k, v, k_scale, v_scale)
+    _auto_check("write8")
+
+
+def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | None = None, per_row: int | None = None,
+                 lens_out: torch.Tensor | None = None, n_free_out: torch.Tensor | None = None) -> dict:
+    """Pages and slots for `new` int32 [B] more tokens of requests that hold `lens` int32 [B] tokens, built on
+    the device without a host synchronisation.  Not in the reference, whose caller counts on the host.
+
+    page_table int32 [B,max_pages] receives the pages of new blocks, taken from the top of the stack
+    free_pages int32 [pages] with n_free int32 [1] entries.  A request that does not fit (into max_pages, into
+    the slot list, or into what earlier requests left of the stack) is refused as a whole.
+    Slots and positions: packed, request after request, in n_tokens places, or with per_row in a padded
+    [B,per_row] list; -1 in places without a token.
+    Returns dict(slots int64, positions int32, granted bool [B], lens, n_free); the last two are new tensors unless
+    lens_out / n_free_out are given, which may be lens and n_free themselves."""
+    if (n_tokens is None) == (per_row is None):
+        raise ValueError("extend_pages: either n_tokens (packed) or per_row (padded)")
+    if per_row is not None and per_row < 1:
+        raise ValueError("extend_pages: per_row >= 1")
+    slots, positions, granted, lens2, n2 = ext().extend_pages(lens, new, page_table, free_pages, n_free, n_tokens or 0,
+                                                              per_row or 0, lens_out, n_free_out)
+    return {"slots": slots, "positions": positions, "granted": granted, "lens": lens2, "n_free": n2}
+
+
+def release_pages(done, lens, page_table, free_pages, n_free, *, lens_out: torch.Tensor | None = None,
+                  n_free_out: torch.Tensor | None = None) -> dict:
+    """The pages of the requests marked in `done` (bool or uint8 [B]) go back to the stack of
+    `extend_pages` and their lengths become 0 (the table is left as it is).  Returns dict(lens, n_free), new
+    tensors unless lens_out / n_free_out are given."""
+    lens2, n2 = ext().release_pages(done, lens, page_table, free_pages, n_free, lens_out, n_free_out)
+    return {"lens": lens2, "n_free": n2}

@@ -1,0 +1,525 @@
+"""The 8-bit cache: attention, write, page tables, and a run of them together, against plain restatements.
+
+Tolerances.  A score is an fp32 sum of D products on the tensor cores; taking every addition as truncated (2^-23
+of the partial sums) its error is at most d = D 2^-23 S + 2^-21 |s| with S = scale sum |q k| >= |s| (the second
+part: the product with the scales, the exponent's argument).  A weight is then off by 2 d relative to the
+normaliser, by 2^-20 from the exponential and the two 11-bit parts that hold it, and the sums over tokens and
+blocks add (64 + blocks) 2^-23 of sum p |v|.  16-bit outputs add half a step (bf16 2^-8, fp16 2^-11)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from kvskip_b200 import kvskip as K
+from kvskip_b200.cache import PagedKV8
+from kvskip_b200.graph import StepGraph
+from tests import cache8_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TILE = 64
+
+
+def _cpu(t):
+    return t.float().cpu() if t.dtype in (torch.float8_e4m3fn,) else t.cpu()
+
+
+def _codes(shape, kind, gen):
+    """Codes of values with a mean and a spread of their own per channel."""
+    x = torch.randn(*shape, generator=gen) * torch.exp(0.5 * torch.randn(shape[-1], generator=gen)) \
+        + 0.5 * torch.randn(shape[-1], generator=gen)
+    x = x * (60.0 if kind == "e4m3" else 25.0)
+    return x.clamp(-440, 440).to(torch.float8_e4m3fn) if kind == "e4m3" else x.round().clamp(-127, 127).to(torch.int8)
+
+
+def _case(lens, Hkv, G, D, kind, qtype, layout, seed=0, T=None, poison=True):
+    """CPU tensors of a case; rows behind a length hold NaN codes (e4m3) or 127s, spare pages and their scales NaN."""
+    gen = torch.Generator().manual_seed(seed)
+    B, T = len(lens), T or max(max(lens), 1)
+    nb = -(-T // TILE)
+    q = (1.5 * torch.randn(B, Hkv * G, D, generator=gen)).to(qtype)
+    scale_of = lambda *s: torch.exp(0.3 * torch.randn(*s, generator=gen)) / (60.0 if kind == "e4m3" else 25.0)  # noqa: E731
+    bad = 0x7F
+    c = {"q": q, "lens": torch.tensor(lens, dtype=torch.int32), "scale": 1 / math.sqrt(D), "table": None, "nb": nb}
+    if layout == "paged":
+        n = sum(-(-x // TILE) for x in lens) + 3
+        order = torch.randperm(n, generator=gen).tolist()
+        table = torch.full((B, nb), -7, dtype=torch.int32)
+        ends = []
+        for b, x in enumerate(lens):
+            for j in range(-(-x // TILE)):
+                table[b, j] = order.pop()
+            if x % TILE:
+                ends.append((int(table[b, x // TILE]), x % TILE))
+        c["table"] = table
+        for name in ("k", "v"):
+            codes, s = _codes((n, Hkv, TILE, D), kind, gen), scale_of(n, Hkv)
+            if poison:
+                for pg, r in ends:
+                    codes.view(torch.uint8)[pg, :, r:] = bad
+                codes.view(torch.uint8)[order] = bad
+                s[order] = math.nan
+            c[name], c[name + "s"] = codes, s
+    else:
+        for name in ("k", "v"):
+            codes, s = _codes((B, Hkv, T, D), kind, gen), scale_of(B, Hkv, nb)
+            if poison:
+                for b, x in enumerate(lens):
+                    codes.view(torch.uint8)[b, :, x:] = bad
+                    s[b, :, -(-x // TILE):] = math.nan
+            c[name], c[name + "s"] = codes, s
+    return c
+
+
+def _dev(c):
+    return {n: (t.to(DEV) if isinstance(t, torch.Tensor) else t) for n, t in c.items()}
+
+
+def _run(d, plan=None, stats=False, **kw):
+    return K.decode8(d["q"], d["k"], d["v"], d["ks"], d["vs"], d["scale"], lens=d["lens"], page_table=d["table"],
+                     plan=plan, stats=stats, out_f32=True, **kw)
+
+
+def _check(r, ref, D, nb, qtype):
+    qk = ref["qk"][..., None]
+    live = torch.isfinite(ref["lse"])
+    s_max = qk                                                   # |s| <= S
+    d = D * 2.0 ** -23 * qk + 2.0 ** -21 * s_max
+    rel = 2 * d + 2.0 ** -20 + (64 + nb) * 2.0 ** -23
+    tol = rel * ref["mag"]
+    o32, out, lse = r["out_f32"].double().cpu(), r["out"].double().cpu(), r["lse"].double().cpu()
+    assert ((o32 - ref["out"]).abs() <= tol).all(), float(((o32 - ref["out"]).abs() - tol).max())
+    half = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[qtype]
+    assert ((out - ref["out"]).abs() <= tol + half * (ref["out"].abs() + tol) + 2.0 ** -25).all()
+    assert r["out"].dtype == qtype
+    assert torch.equal(torch.isneginf(lse), ~live)
+    tl = (rel[..., 0] + 2.0 ** -22 * ref["lse"].abs())[live]
+    assert ((lse - ref["lse"])[live].abs() <= tl).all()
+    if "blk_max" in r:
+        bm, bs = r["blk_max"].double().cpu(), r["blk_sum"].double().cpu()
+        seen = torch.isfinite(ref["blk_max"])
+        assert torch.equal(torch.isfinite(bm), seen) and (bs[~seen] == 0).all()
+        dd = d.expand_as(bm)
+        assert ((bm - ref["blk_max"])[seen].abs() <= dd[seen]).all()
+        assert ((bs - ref["blk_sum"])[seen].abs() <= (rel.expand_as(bs) * ref["blk_sum"])[seen]).all()
+
+
+LENS = [0, 1, 63, 64, 65, 128, 1000, 2047]
+
+
+@pytest.mark.parametrize("layout", ["paged", "contiguous"])
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("Hkv,G,D,qtype", [(8, 4, 128, torch.bfloat16), (2, 8, 64, torch.float16),
+                                           (3, 5, 128, torch.float16), (1, 16, 64, torch.bfloat16),
+                                           (2, 9, 128, torch.bfloat16), (4, 1, 64, torch.bfloat16)])
+def test_decode8_lengths_and_head_layouts(layout, kind, Hkv, G, D, qtype):
+    c = _case(LENS, Hkv, G, D, kind, qtype, layout, seed=Hkv * 100 + G)
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], LENS, c["table"])
+    r = _run(_dev(c), stats=True)
+    _check(r, ref, D, c["nb"], qtype)
+    a = _run(_dev(c), stats=True)
+    assert all(torch.equal(r[n], a[n]) for n in ("out", "out_f32", "lse", "blk_max", "blk_sum"))
+    assert K.ext().device_status() == 0
+
+
+@pytest.mark.parametrize("lens", [[1], [64], [65], [0], [0, 0, 5], [4097], [20000], [300] * 70, [130, 0] * 300])
+def test_decode8_work_split(lens):
+    """One short request, one long one over every SM, many of a few blocks, batches larger than a CTA has threads."""
+    Hkv = 2 if len(lens) > 4 else 8
+    c = _case(lens, Hkv, 4, 128, "e4m3", torch.bfloat16, "paged", seed=len(lens))
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], lens, c["table"])
+    _check(_run(_dev(c)), ref, 128, c["nb"], torch.bfloat16)
+    # a bound that is smaller than the table, and one-token clamps
+    m = max(1, max(lens) - 3)
+    short = [min(x, m) for x in lens]
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], short, c["table"])
+    _check(_run(_dev(c), max_len=m), ref, 128, c["nb"], torch.bfloat16)
+
+
+@pytest.mark.parametrize("kind,layout,G", [("e4m3", "paged", 4), ("int8", "contiguous", 8), ("e4m3", "contiguous", 12)])
+def test_decode8_block_lists(kind, layout, G):
+    lens, Hkv, D = [1500, 64, 0, 777, 1], 3, 128
+    c = _case(lens, Hkv, G, D, kind, torch.bfloat16, layout, seed=5)
+    nb = c["nb"]
+    gen = torch.Generator().manual_seed(3)
+    keep = torch.rand(len(lens), Hkv, nb, generator=gen) < 0.4
+    keep[0, 1] = False                                           # an empty list
+    keep[0, 2] = True                                            # every block
+    keep[3, :, nb - 1] = True                                    # a block behind the length: no tokens
+    lists = {(b, h): torch.nonzero(keep[b, h])[:, 0].tolist() for b in range(len(lens)) for h in range(Hkv)}
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], lens, c["table"], lists)
+    d = _dev(c)
+    plan = K.make_plan(keep.to(DEV))
+    _check(_run(d, plan=plan, stats=True), ref, D, nb, torch.bfloat16)
+    # entries behind the count are not used, whatever they hold
+    idx = plan.block_idx.clone()
+    idx[torch.arange(nb, device=DEV)[None, None] >= plan.block_cnt[..., None]] = 1 << 29
+    _check(_run(d, plan=K.Plan(idx, plan.block_cnt, nb, nb), stats=True), ref, D, nb, torch.bfloat16)
+
+
+def test_decode8_strides_and_optional_lengths():
+    B, Hkv, G, D, T = 2, 4, 4, 128, 333
+    c = _case([T] * B, Hkv, G, D, "e4m3", torch.bfloat16, "contiguous", seed=9)
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], [T] * B)
+    d = _dev(c)
+    # token-major cache, block-major scales, q as [B,Hq,1,D] out of a wider buffer, no lens
+    def widen(t):
+        w = torch.zeros(B, T + 5, Hkv, D, dtype=torch.uint8, device=DEV).view(t.dtype)
+        w.view(torch.uint8)[:, :T] = t.transpose(1, 2).view(torch.uint8)
+        return w.transpose(1, 2)[:, :, :T]
+    ks = torch.zeros(6, B, Hkv, device=DEV).permute(1, 2, 0)
+    vs = torch.zeros_like(ks)
+    ks[:, :, :], vs[:, :, :] = d["ks"], d["vs"]
+    wide = torch.zeros(B, Hkv * G, 2, 2 * D, dtype=torch.bfloat16, device=DEV)
+    wide[:, :, 1, :D] = d["q"]
+    q = wide[:, :, 1:, :D]
+    assert q.dim() == 4 and not q.is_contiguous()
+    r = K.decode8(q, widen(d["k"]), widen(d["v"]), ks, vs, c["scale"], out_f32=True)
+    _check(r, ref, D, c["nb"], torch.bfloat16)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_decode8_extreme_values(kind):
+    """Block scales far apart, a bf16 q far outside fp16, a query of zeros, one dominant token."""
+    lens, Hkv, G, D = [500, 200], 2, 4, 64
+    c = _case(lens, Hkv, G, D, kind, torch.bfloat16, "contiguous", seed=2)
+    for b, x in enumerate(lens):
+        n = -(-x // TILE)
+        c["vs"][b, :, :n] *= torch.logspace(-12, 12, n)[None]
+    c["q"][0, 0] *= 2.0 ** 60
+    c["ks"][0, 0] *= 2.0 ** -60                                     # scores as before
+    c["q"][0, 1:4] = c["q"][0, 1:4] * 2.0 ** 57
+    c["q"][1, 2] = 0
+    # a dominant token: its key along q
+    c["k"][1, 1, 100] = (c["q"][1, 5].float().sign() * 100).to(c["k"].dtype)
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], lens)
+    _check(_run(_dev(c), stats=True), ref, D, c["nb"], torch.bfloat16)
+
+
+def test_decode8_nan_stays_in_its_row():
+    lens, Hkv, G, D = [300, 300], 2, 4, 128
+    c = _case(lens, Hkv, G, D, "e4m3", torch.bfloat16, "paged", seed=4)
+    d = _dev(c)
+    clean = _run(d)
+    d["k"].view(torch.uint8)[int(c["table"][0, 1]), 0, 7, 3] = 0x7F     # a NaN in a key that is read
+    r = _run(d)
+    assert torch.isnan(r["out_f32"][0, :G]).all() and torch.isnan(r["lse"][0, :G]).all()
+    assert torch.equal(r["out_f32"][0, G:], clean["out_f32"][0, G:]) and torch.equal(r["out_f32"][1], clean["out_f32"][1])
+
+
+def test_decode8_pages_outside_the_pool_read_as_zeros():
+    lens = [200, 70]
+    c = _case(lens, 2, 4, 128, "e4m3", torch.bfloat16, "paged", seed=6)
+    c["table"][0, 1] = -1
+    c["table"][1, 0] = c["k"].shape[0]
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], lens, c["table"])
+    _check(_run(_dev(c), stats=True), ref, 128, c["nb"], torch.bfloat16)
+
+
+def test_decode8_offsets_beyond_32_bits():
+    """Pages whose byte offset, and a contiguous cache whose head offset, pass 2^32."""
+    D, lens = 128, [150]
+    c = _case(lens, 1, 4, D, "e4m3", torch.bfloat16, "paged", seed=8, poison=False)
+    n = (1 << 32) // (TILE * D) + 64
+    far = torch.tensor([n - 1, n - 9, n - 33], dtype=torch.int32)
+    pools = {}
+    for name in ("k", "v"):
+        big = torch.empty(n, 1, TILE, D, dtype=torch.uint8, device=DEV)
+        s = torch.zeros(n, 1, device=DEV)
+        for j in range(3):
+            big[int(far[j])] = c[name][int(c["table"][0, j])].view(torch.uint8).to(DEV)
+            s[int(far[j])] = c[name + "s"][int(c["table"][0, j])].to(DEV)
+        pools[name], pools[name + "s"] = big.view(torch.float8_e4m3fn), s
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], lens, c["table"])
+    d = {**_dev(c), **pools, "table": far[None].to(DEV).contiguous()}
+    _check(_run(d), ref, D, 3, torch.bfloat16)
+    # and the write: the same token again, far out
+    x = torch.randn(2, 1, D, device=DEV, dtype=torch.bfloat16)
+    slots = torch.tensor([int(far[0]) * TILE, int(far[0]) * TILE + 1], device=DEV)
+    K.write8(x, -x, slots, d["k"], d["v"], d["ks"], d["vs"])
+    got = d["k"][int(far[0]), 0, :2].float() * d["ks"][int(far[0]), 0]
+    assert ((got - x[:, 0].float()).abs() <= 2.0 ** -4 * x[:, 0].float().abs() + 2.0 ** -10 * d["ks"][int(far[0]), 0]).all()
+    assert torch.equal(d["v"][int(far[0]), 0, :2].float(), -d["k"][int(far[0]), 0, :2].float())
+
+
+def test_decode8_streams_and_concurrent_graphs():
+    """Calls on two streams, and two graphs captured on one stream and replayed side by side, do not share anything."""
+    cs = [_dev(_case([20000, 30], 4, 4, 128, "e4m3", torch.bfloat16, "paged", seed=s)) for s in (1, 2)]
+    want = [_run(d) for d in cs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for d, s in zip(cs, streams):
+            with torch.cuda.stream(s):
+                got.append(_run(d))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g["out_f32"], w["out_f32"]) and torch.equal(g["lse"], w["lse"])
+    graphs, outs = [], []
+    for d in cs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_run(d))
+        graphs.append(g)
+    for _ in range(5):
+        for o in outs:
+            o["out_f32"].zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o["out_f32"], w["out_f32"]) and torch.equal(o["lse"], w["lse"])
+
+
+# ------------------------------------------------------------------------------------------ write8
+def _pool(n, Hkv, D, kind, gen):
+    return _codes((n, Hkv, TILE, D), kind, gen), torch.exp2(torch.randint(-8, -2, (n, Hkv), generator=gen).float())
+
+
+def _write_both(x, slots, codes, scales, kind, k4=None):
+    """The call and the restatement on copies; the codes of K and V (= -x: the same scales) have to be equal."""
+    want_c, want_s = codes.view(torch.uint8).numpy().copy(), scales.numpy().copy()
+    R.write_ref(x.float().numpy(), slots.reshape(-1).tolist(), want_c, want_s, kind)
+    k, v, ks, vs = codes.to(DEV), codes.clone().to(DEV), scales.to(DEV), scales.clone().to(DEV)
+    xd = x.to(DEV)
+    a, b = (xd, xd) if k4 is None else (k4(xd), k4(xd))
+    K.write8(a, b, slots.to(DEV), k, v, ks, vs)
+    for got_c, got_s in ((k, ks), (v, vs)):
+        assert np.array_equal(got_s.cpu().numpy(), want_s, equal_nan=True)
+        assert _same_codes(got_c.view(torch.uint8).cpu().numpy(), want_c, kind)
+    return k, ks
+
+
+def _same_codes(got, want, kind):
+    """Equal bits; the two e4m3 codes of a NaN (0x7F, 0xFF) count as one, a NaN has no sign."""
+    if kind == "e4m3":
+        got, want = np.where(got == 0xFF, 0x7F, got), np.where(want == 0xFF, 0x7F, want)
+    return bool(np.array_equal(got, want))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("qtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("runs", [[(0, 1)], [(0, 64)], [(3, 61)], [(63, 1)], [(5, 1), (0, 64), (0, 9), (60, 4), (0, 1)],
+                                  [(r % 64, 1) for r in range(0, 200, 3)], [(0, 64)] * 20 + [(0, 7)],
+                                  [(17, 30), (0, 50)] * 8])
+def test_write8_matches_the_restatement(D, kind, qtype, runs):
+    Hkv, gen = 3, torch.Generator().manual_seed(len(runs) * D)
+    codes, scales = _pool(len(runs) + 2, Hkv, D, kind, gen)
+    pages = torch.randperm(len(runs) + 2, generator=gen).tolist()
+    slots = torch.tensor([pages[i] * TILE + r + j for i, (r, n) in enumerate(runs) for j in range(n)])
+    x = torch.randn(len(slots), Hkv, D, generator=gen) * torch.exp2(torch.randint(-6, 7, (len(slots), 1, 1), generator=gen).float())
+    _write_both(x.to(qtype), slots, codes, scales, kind)
+    assert K.ext().device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("qtype", [torch.bfloat16, torch.float16])
+def test_write8_special_values(kind, qtype):
+    Hkv, D, gen = 2, 64, torch.Generator().manual_seed(1)
+    codes, scales = _pool(8, Hkv, D, kind, gen)
+    x = torch.randn(40, Hkv, D, generator=gen)
+    x[0, 0, :4] = torch.tensor([math.inf, -math.inf, math.nan, 0.0])
+    x[1] = 0.0                                        # a block of zeros
+    x[2, 0] = math.nan                                # nothing finite
+    x[3, 1] = 2.0 ** -24                              # the smallest fp16 number
+    x[4] = torch.finfo(qtype).max * (1 if qtype is torch.float16 else 0.9)
+    x[5, :, :2] = torch.tensor([448.0, 127.0])        # exactly the largest code
+    x[5, :, 2:] = 0.25
+    x[6, :, :2] = torch.tensor([450.0, 128.0])        # just above
+    x[7:20, 0, 5] = math.inf
+    slots = torch.tensor([0, 64, 128, 192, 256, 320, 384 + 5] + list(range(448, 448 + 33)))
+    scales[6, 0], scales[6, 1] = math.nan, -3.0       # a scale that is none, in front of row 5
+    _write_both(x.to(qtype), slots, codes, scales, kind)
+
+
+def test_write8_growing_a_block_token_by_token():
+    """Every token of a block in a call of its own, larger and larger values: the scale grows and the codes of the earlier
+    ones are rounded again; values stay within half a step of each rounding."""
+    Hkv, D = 2, 128
+    for kind in ("e4m3", "int8"):
+        gen = torch.Generator().manual_seed(7)
+        codes, scales = _pool(2, Hkv, D, kind, gen)
+        want_c, want_s = codes.view(torch.uint8).numpy().copy(), scales.numpy().copy()
+        k, ks = codes.to(DEV), scales.to(DEV)
+        v, vs = k.clone(), ks.clone()
+        x = torch.randn(64, Hkv, D, generator=gen).to(torch.bfloat16) * torch.exp2(torch.arange(64) / 9)[:, None, None]
+        x = x.to(torch.bfloat16)
+        for r in range(64):
+            s = torch.tensor([64 + r], device=DEV)
+            K.write8(x[r:r + 1].to(DEV), x[r:r + 1].to(DEV), s, k, v, ks, vs)
+            R.write_ref(x[r:r + 1].float().numpy(), [64 + r], want_c, want_s, kind)
+        assert np.array_equal(k.view(torch.uint8).cpu().numpy(), want_c) and np.array_equal(ks.cpu().numpy(), want_s)
+        got = k[1].float().cpu() * ks[1].cpu()[:, None, None]
+        err = (got - x.float().transpose(0, 1)).abs()
+        s = ks[1].cpu()[:, None, None]
+        if kind == "int8":      # half a step for each rounding, each time of at most half the next scale: < 1 step
+            assert (err <= s).all()
+        else:                   # one rounding of 2^-4; below 2^-6 of the scale, half a step 2^-10 and as much for the later ones
+            assert (err <= 2.0 ** -4 * x.float().transpose(0, 1).abs() + 2.0 ** -9 * s).all()
+
+
+def test_write8_layouts():
+    """[B,Hkv,S,D] views into a contiguous cache whose capacity is no multiple of a block, and padding tokens."""
+    B, Hkv, S, D, T = 3, 2, 70, 64, 200
+    nb, gen = 4, torch.Generator().manual_seed(3)
+    x = torch.randn(B, S, Hkv, D, generator=gen).to(torch.bfloat16)
+    start = [0, 10, 129]
+    slots = torch.full((B, S), -1)
+    for b in range(B):
+        n = S if b != 1 else 33                                  # row 1 is padded
+        slots[b, :n] = b * nb * TILE + start[b] + torch.arange(n)
+    codes, scales = _pool(B * nb, Hkv, D, "e4m3", gen)
+    want_c, want_s = codes.view(torch.uint8).numpy().copy(), scales.numpy().copy()
+    R.write_ref(x.reshape(-1, Hkv, D).float().numpy(), slots.reshape(-1).tolist(), want_c, want_s, "e4m3")
+    cap = torch.zeros(B, Hkv, nb * TILE, D, dtype=torch.uint8, device=DEV)
+    cap.view(B, Hkv, nb, TILE, D)[:] = codes.view(torch.uint8).view(B, nb, Hkv, TILE, D).transpose(1, 2).to(DEV)
+    before = cap.clone()
+    k = cap.view(torch.float8_e4m3fn)[:, :, :T]
+    v = k.clone()
+    ks = scales.view(B, nb, Hkv).transpose(1, 2).to(DEV)
+    vs = ks.clone()
+    xd = x.transpose(1, 2).to(DEV)
+    wide = torch.zeros(B, Hkv, S, 2 * D, dtype=torch.bfloat16, device=DEV)
+    wide[..., :D] = xd
+    K.write8(wide[..., :D], xd.contiguous(), slots.to(DEV), k, v, ks, vs)
+    want = torch.from_numpy(want_c).view(B, nb, Hkv, TILE, D).transpose(1, 2).reshape(B, Hkv, nb * TILE, D)
+    assert torch.equal(cap[:, :, :T].cpu(), want[:, :, :T])
+    assert torch.equal(cap[:, :, T:], before[:, :, T:])
+    assert torch.equal(v.view(torch.uint8).cpu(), want[:, :, :T])
+    assert np.array_equal(ks.cpu().numpy(), torch.from_numpy(want_s).view(B, nb, Hkv).transpose(1, 2).numpy())
+
+
+def test_write8_skips_and_reports_bad_slots():
+    Hkv, D, gen = 2, 128, torch.Generator().manual_seed(3)
+    codes, scales = _pool(4, Hkv, D, "int8", gen)
+    x = torch.randn(6, Hkv, D, generator=gen).to(torch.bfloat16)
+    _write_both(x, torch.tensor([5, 4 * TILE, 70, -1, 1 << 40, 130]), codes, scales, "int8")
+    assert K.ext().device_status() == 0x302
+    _write_both(x, torch.tensor([5, 5, 6, 64, 130, 129]), codes, scales, "int8")         # a second run of one block
+    assert K.ext().device_status() == 0x303
+    assert K.ext().device_status() == 0
+    # a contiguous cache: rows behind the last one it has room for
+    k = torch.zeros(1, Hkv, 100, D, dtype=torch.int8, device=DEV)
+    s = torch.ones(1, Hkv, 2, device=DEV)
+    K.write8(x[:2].to(DEV), x[:2].to(DEV), torch.tensor([99, 100], device=DEV), k, k.clone(), s, s.clone())
+    assert K.ext().device_status() == 0x302
+    assert (k[:, :, :99] == 0).all() and (k[:, :, 99] != 0).any()
+
+
+# ------------------------------------------------------------------------------------------ pages
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("B,hi,new_hi,pool,mode", [(1, 0, 1, 1.0, "packed"), (1, 130, 500, 1.0, "packed"),
+                                                   (7, 300, 1, 1.0, "row"), (513, 700, 1, 1.0, "row"),
+                                                   (100, 700, 90, 0.6, "packed"), (1500, 300, 70, 0.7, "packed"),
+                                                   (2049, 300, 3, 0.9, "row"), (33, 100, 5000, 1.0, "packed"),
+                                                   (40, 100, 4000, 0.5, "row")])
+def test_extend_and_release_pages(B, hi, new_hi, pool, mode, inplace):
+    gen = torch.Generator().manual_seed(B + new_hi)
+    lens = torch.randint(0, hi + 1, (B,), generator=gen).tolist()
+    new = torch.randint(0 if B > 1 else 1, new_hi + 1, (B,), generator=gen).tolist()
+    if B > 8:
+        new[3], new[5] = -4, 0
+    cap = -(-(hi + new_hi) // TILE) - (1 if B > 50 else 0)          # some requests run into the table's end
+    lens = [min(x, cap * TILE) for x in lens]
+    have = sum(-(-x // TILE) for x in lens)
+    extra = sum(-(-(x + max(0, n)) // TILE) for x, n in zip(lens, new)) - have
+    pages = have + max(1, int(extra * pool))
+    order = torch.randperm(pages, generator=gen).tolist()
+    table = [[-1] * cap for _ in range(B)]
+    for b in range(B):
+        for j in range(-(-lens[b] // TILE)):
+            table[b][j] = order.pop()
+    n_free, free = len(order), order + [-9] * (pages - len(order))
+    kw = {"per_row": max(max(new) - (1 if B > 1000 else 0), 1)} if mode == "row" else {"n_tokens": sum(max(0, n) for n in new) + (5 if B != 100 else -20)}
+    want = R.extend_ref(lens, new, table, free, n_free, **kw)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    ld, td, fd, nd = i32(lens), i32(table), i32(free), i32([n_free])
+    out = {"lens_out": ld, "n_free_out": nd} if inplace else {}
+    r = K.extend_pages(ld, i32(new), td, fd, nd, **kw, **out)
+    assert r["slots"].flatten().tolist() == want[0] and r["positions"].flatten().tolist() == want[1]
+    assert r["granted"].tolist() == want[2] and r["lens"].tolist() == want[3] and r["n_free"].tolist() == [want[5]]
+    assert td.tolist() == want[4] and fd.tolist() == free
+    assert (ld.tolist() == lens or inplace) and (nd.tolist() == [n_free] or inplace)
+    done = torch.rand(B, generator=gen) < 0.5
+    back = R.release_ref(done.tolist(), want[3], want[4], free, want[5])
+    ld, nd = r["lens"], r["n_free"]
+    out = {"lens_out": ld, "n_free_out": nd} if inplace else {}
+    r = K.release_pages(done.to(DEV), ld, td, fd, nd, **out)
+    assert r["lens"].tolist() == back[0] and fd.tolist() == back[1] and r["n_free"].tolist() == [back[2]]
+    assert td.tolist() == want[4]
+
+
+# ------------------------------------------------------------------------------------------ together
+@pytest.mark.parametrize("graph", [False, True], ids=["launches", "captured"])
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+def test_serving_loop(kind, graph):
+    """Requests come and go: prompts are admitted, every live one grows by a token a step, finished ones give their
+    pages back to later ones.  The captured form replays extend, write and attention from one graph."""
+    B, Hkv, G, D, steps = 5, 2, 4, 128, 40
+    gen = torch.Generator().manual_seed(11)
+    cache = PagedKV8(24, B, Hkv, D, 512, DEV, dtype=R.KINDS[kind])
+    truth = [torch.zeros(Hkv, 0, D) for _ in range(B)], [torch.zeros(Hkv, 0, D) for _ in range(B)]
+    rand = lambda *s: torch.randn(*s, generator=gen).to(torch.bfloat16)  # noqa: E731
+
+    def admit(prompts):
+        new = torch.tensor(prompts, dtype=torch.int32)
+        k, v = rand(sum(prompts), Hkv, D), rand(sum(prompts), Hkv, D)
+        slots = cache.extend(new.to(DEV), n_tokens=sum(prompts))
+        cache.write(k.to(DEV), v.to(DEV), slots)
+        ok, at = cache.granted.tolist(), 0
+        for b, n in enumerate(prompts):
+            if ok[b]:
+                for t, x in zip(truth, (k, v)):
+                    t[b] = torch.cat([t[b], x[at:at + n].float().transpose(0, 1)], 1)
+            at += n
+        return ok
+
+    assert admit([100, 0, 300, 64, 1]) == [True] * 5
+    live = torch.tensor([1, 0, 1, 1, 1], dtype=torch.int32, device=DEV)
+    kb, vb = (torch.zeros(B, Hkv, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    qb = torch.zeros(B, Hkv * G, D, dtype=torch.bfloat16, device=DEV)
+    scale = 1 / math.sqrt(D)
+
+    def launch():
+        cache.append(kb, vb, live)
+        return cache.decode(qb, scale, out_f32=True)
+
+    step = StepGraph(launch, [cache]) if graph else None
+    for t in range(steps):
+        if t == 15:                                       # request 2 ends, request 1 begins in its place in the pool
+            cache.release(torch.tensor([0, 0, 1, 0, 0], dtype=torch.uint8, device=DEV))
+            for x in truth:
+                x[2] = x[2][:, :0]
+            assert admit([0, 333, 0, 0, 0]) == [True] * 5
+            live.copy_(torch.tensor([1, 1, 0, 1, 1], dtype=torch.int32))
+        if t == 25:                                       # a prompt that the pool has no room for
+            assert admit([0, 0, 900, 0, 0])[2] is False
+        k, v, q = rand(B, Hkv, D), rand(B, Hkv, D), rand(B, Hkv * G, D)
+        kb.copy_(k), vb.copy_(v), qb.copy_(q)
+        r = step.step() if graph else launch()
+        ok = cache.granted.tolist()
+        for b in range(B):
+            if live[b] and ok[b]:
+                for x, y in zip(truth, (k, v)):
+                    x[b] = torch.cat([x[b], y[b].float()[:, None]], 1)
+        lens = cache.lens.tolist()
+        assert lens == [x.shape[1] for x in truth[0]]
+        ref = R.decode_f64(q, _cpu(cache.k), _cpu(cache.v), cache.k_scale.cpu(), cache.v_scale.cpu(), scale, lens,
+                           cache.table.cpu())
+        _check(r, ref, D, cache.max_pages, torch.bfloat16)
+    # what the pool holds is the tokens that went in, to 8 bits: int8 a step, e4m3 2^-4 and its smallest values
+    for b in range(B):
+        for got, t in zip(cache.gather(b), truth):
+            if not t[b].numel():
+                continue
+            top = t[b].abs().max()
+            bound = 2 * top / 127 if kind == "int8" else 2.0 ** -4 * t[b].abs() + top * 2.0 ** -16
+            assert ((got.cpu() - t[b]).abs() <= bound).all()
+    assert K.ext().device_status() == 0
+    if graph:
+        assert step.captures == 1 and step.replays == steps - 1

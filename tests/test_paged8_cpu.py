@@ -1,0 +1,134 @@
+"""The 8-bit cache without a GPU: what is refused before anything runs, the C entry points' argument checks, and the
+layout of their parameter blocks."""
+import ctypes
+import subprocess
+import tempfile
+from pathlib import Path
+
+import pytest
+import torch
+
+from kvskip_b200 import cabi
+from kvskip_b200 import kvskip as K
+from kvskip_b200.cache import PagedKV8
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from kvskip_b200 import build
+    build.build_lib()
+    lib = ctypes.CDLL(str(build.LIB))
+    lib.kvskip_last_error.restype = ctypes.c_char_p
+    lib.kvskip_decode8_work_bytes.restype = ctypes.c_int64
+    return lib
+
+
+def test_parameter_blocks_match_the_header():
+    names = {"kvskip_decode8_params": cabi.Decode8Params, "kvskip_write8_params": cabi.Write8Params,
+             "kvskip_pages_params": cabi.PagesParams}
+    body = "".join(f'printf("%zu ", sizeof({n}));' for n in names)
+    for n, c in names.items():
+        for f, _ in c._fields_:
+            body += f'printf("%zu ", offsetof({n}, {f}));'
+    src = f'#include <stdio.h>\n#include <stddef.h>\n#include "kvskip_b200.h"\nint main(){{{body}return 0;}}\n'
+    with tempfile.TemporaryDirectory() as d:
+        c = Path(d) / "s.c"
+        c.write_text(src)
+        subprocess.run(["/usr/bin/gcc", "-I", str(ROOT / "include"), str(c), "-o", str(Path(d) / "s")], check=True)
+        out = subprocess.run([str(Path(d) / "s")], capture_output=True, text=True, check=True).stdout.split()
+    want = [ctypes.sizeof(c) for c in names.values()] + [getattr(c, f).offset for c in names.values() for f, _ in c._fields_]
+    assert [int(x) for x in out] == want
+
+
+def _decode_params(**kw):
+    p = cabi.Decode8Params()
+    base = dict(q=4096, k=4096, v=4096, k_scale=4096, v_scale=4096, out=4096, lse=4096, work=4096, q_sb=512, q_sh=128,
+                k_sb=65536, k_sh=8192, k_st=128, v_sb=65536, v_sh=8192, v_st=128, kind=0, B=1, Hq=32, Hkv=8, D=128,
+                T=100, nb=2, lens=4096)
+    for n, x in {**base, **kw}.items():
+        setattr(p, n, x)
+    return p
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(D=96), b"head dim"), (dict(kind=2), b"kind"), (dict(B=0), b"bad B"), (dict(Hq=30), b"bad B"),
+    (dict(Hq=17 * 8), b"at most 16"), (dict(T=0, nb=0), b"bad B"), (dict(q=0), b"required"), (dict(work=0), b"required"),
+    (dict(nb=3), b"nb must be"), (dict(block_idx=4096), b"go together"), (dict(blk_max=4096), b"go together"),
+    (dict(page_table=4096, max_pages=1, num_pages=9), b"page table"), (dict(page_table=4096, max_pages=2), b"page table"),
+    (dict(page_table=4096, max_pages=2, num_pages=9, lens=0), b"needs lens"), (dict(q=4100), b"8-byte"),
+    (dict(q_sh=130), b"8-byte"), (dict(k=4104), b"16-byte"), (dict(v_st=136), b"16"), (dict(work=4100), b"misaligned"),
+    (dict(B=1 << 20, T=1 << 20, nb=1 << 14), b"2^31")])
+def test_decode8_entry_refuses(lib, change, text):
+    assert lib.kvskip_launch_decode8(ctypes.byref(_decode_params(**change)), None) < 0
+    assert text in lib.kvskip_last_error()
+
+
+def test_null_blocks_and_sizes(lib):
+    for n in ("decode8", "write8", "extend_pages", "release_pages"):
+        assert getattr(lib, f"kvskip_launch_{n}")(None, None) == -1 and b"null" in lib.kvskip_last_error()
+    assert lib.kvskip_decode8_work_bytes(17, 128) == 0 and lib.kvskip_decode8_work_bytes(4, 96) == 0
+    assert lib.kvskip_decode8_work_bytes(16, 128) > lib.kvskip_decode8_work_bytes(4, 128) > 0
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(D=32), b"head dim"), (dict(kind=7), b"kind"), (dict(inner=0), b"bad n"), (dict(blocks=0), b"bad n"),
+    (dict(slots=0), b"required"), (dict(k_new=4104), b"16-byte"), (dict(vn_sh=100), b"16-byte"), (dict(k=4100), b"8-byte"),
+    (dict(v_st=132), b"8-byte"), (dict(Hkv=70000), b"grid")])
+def test_write8_entry_refuses(lib, change, text):
+    p = cabi.Write8Params()
+    base = dict(k_new=4096, v_new=4096, kn_si=1024, kn_sh=128, vn_si=1024, vn_sh=128, n=4, inner=4, slots=4096, k=4096,
+                v=4096, k_sb=65536, k_sh=8192, k_st=128, v_sb=65536, v_sh=8192, v_st=128, k_scale=4096, v_scale=4096,
+                kind=0, Hkv=8, D=128, blocks=1, tokens=64, num_blocks=5)
+    for n, x in {**base, **change}.items():
+        setattr(p, n, x)
+    assert lib.kvskip_launch_write8(ctypes.byref(p), None) < 0
+    assert text in lib.kvskip_last_error()
+
+
+@pytest.mark.parametrize("fn,change,text", [
+    ("extend_pages", dict(lens=0), b"required"), ("extend_pages", dict(new_=0), b"required"),
+    ("extend_pages", dict(slots=0), b"required"), ("extend_pages", dict(B=0), b">= 1"),
+    ("extend_pages", dict(per_row=3), b"per_row"), ("extend_pages", dict(n_tokens=-1), b"n_tokens"),
+    ("extend_pages", dict(max_pages=1 << 27), b"2^31"), ("release_pages", dict(done=0), b"done"),
+    ("release_pages", dict(free_pages=0), b"required")])
+def test_pages_entries_refuse(lib, fn, change, text):
+    p = cabi.PagesParams()
+    base = dict(lens=4096, new_=4096, done=4096, table=4096, free_pages=4096, n_free=4096, lens_out=4096,
+                n_free_out=4096, slots=4096, positions=4096, granted=4096, n_tokens=4, B=2, max_pages=4, num_free=9)
+    for n, x in {**base, **change}.items():
+        setattr(p, n, x)
+    assert getattr(lib, f"kvskip_launch_{fn}")(ctypes.byref(p), None) < 0
+    assert text in lib.kvskip_last_error()
+
+
+def test_front_end_refuses_cpu_tensors():
+    k = torch.zeros(3, 2, 64, 64, dtype=torch.float8_e4m3fn)
+    s = torch.ones(3, 2)
+    i = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        K.decode8(torch.zeros(1, 8, 64, dtype=torch.bfloat16), k, k, s, s, 1.0, lens=i, page_table=i[None])
+    x = torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        K.write8(x, x, torch.zeros(1, dtype=torch.int64), k, k.clone(), s, s.clone())
+    with pytest.raises(RuntimeError, match="CUDA"):
+        K.extend_pages(i, i, i[None], i, i, n_tokens=1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        K.release_pages(i.bool(), i, i[None], i, i)
+
+
+def test_front_end_argument_errors():
+    i = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="n_tokens"):
+        K.extend_pages(i, i, i[None], i, i)
+    with pytest.raises(ValueError, match="n_tokens"):
+        K.extend_pages(i, i, i[None], i, i, n_tokens=1, per_row=1)
+    with pytest.raises(ValueError, match="per_row"):
+        K.extend_pages(i, i, i[None], i, i, per_row=0)
+    with pytest.raises(ValueError, match="int8"):
+        PagedKV8(1, 1, 1, 64, 64, "cpu", dtype=torch.uint8)
+    with pytest.raises(ValueError, match="head dim"):
+        PagedKV8(1, 1, 1, 96, 64, "cpu")
+    with pytest.raises(ValueError, match="at least 1"):
+        PagedKV8(0, 1, 1, 64, 64, "cpu")
