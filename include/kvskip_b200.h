@@ -331,7 +331,7 @@ typedef struct kvskip_decode8_params {
   float* lse;     /* [B,Hq] natural-log log-sum-exp */
   float* blk_max; /* optional (both or none) [B,Hq,nb] */
   float* blk_sum;
-  void* work;     /* kvskip_decode8_work_bytes() bytes, 16-byte aligned, contents irrelevant */
+  void* work;     /* kvskip_decode8_work_bytes() bytes, 16-byte aligned, contents irrelevant; of this call alone */
 } kvskip_decode8_params;
 
 /* Attention of one token per sequence over the 8-bit cache, Hq = G * Hkv with 1 <= G <= 16.  Lengths are
@@ -339,7 +339,7 @@ typedef struct kvskip_decode8_params {
  * out = 0 and lse = -inf.  Rows of a block behind the length are never used, whatever they hold.  Block
  * statistics as in kvskip_launch_decode (-inf / 0 on blocks that are not read).  A page table entry
  * outside the pool reads as zeros; a list entry outside the sequence reads nothing. */
-int64_t kvskip_decode8_work_bytes(int G, int D);
+int64_t kvskip_decode8_work_bytes(const kvskip_decode8_params* p); /* from B, Hq, Hkv, D, nb, block_idx, max_blocks */
 int kvskip_launch_decode8(const kvskip_decode8_params* p, void* stream);
 
 typedef struct kvskip_write8_params {

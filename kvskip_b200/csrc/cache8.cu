@@ -65,19 +65,39 @@ int make_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int6
   return KVSKIP_OK;
 }
 
-// Fewest items (blocks of a head) of a CTA: below it fewer CTAs take part.
-constexpr int kMinItems = 4;
+// What of a launch follows from the bound on its items (the lengths are on the device).
+struct Decode8Launch {
+  int ctas, warps, shared;
+};
+template <int D, int MODE>
+Decode8Launch decode8_launch(const kvskip_decode8_params& p) {
+  const int64_t items = static_cast<int64_t>(p.B) * p.Hkv * (p.block_idx ? p.max_blocks : p.nb);
+  Decode8Launch l;
+  l.ctas = static_cast<int>(std::min<int64_t>(kvb_host::num_sms(), items));
+  l.warps = l.ctas * kvb::D8Cfg<D, MODE>::kWarps;
+  l.shared = items >= kvb::D8_SHARE_MIN * static_cast<int64_t>(l.warps);
+  return l;
+}
+template <int D, int MODE>
+int64_t decode8_work(const kvskip_decode8_params& p) {
+  const Decode8Launch l = decode8_launch<D, MODE>(p);
+  const int64_t units = p.block_idx ? static_cast<int64_t>(p.B) * p.Hkv : p.B;
+  return (kvb::d8_piece_base(units) + (l.shared ? 4 : 1) * 2 * static_cast<int64_t>(l.warps) * kvb::D8Cfg<D, MODE>::kPiece) *
+         static_cast<int64_t>(sizeof(float));
+}
 
 template <int KIND, int D, int MODE>
 int launch_decode8(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cudaStream_t stream) {
   using Cfg = kvb::D8Cfg<D, MODE>;
   auto kernel = kvb::decode8_kernel<KIND, D, MODE>;
   if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmem)) return rc;
-  const int64_t items = static_cast<int64_t>(p.B) * p.Hkv * (p.block_idx ? p.max_blocks : p.nb);
-  const int ctas = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(std::min(kvb_host::num_sms(), kvb::D8_MAX_CTAS), (items + kMinItems - 1) / kMinItems)));
-  KVB_CUDA(launch(kernel, dim3(ctas), Cfg::kThreads, Cfg::kSmem, stream, p, maps, kMinItems));
-  if (ctas > 1) KVB_CUDA(launch(kvb::decode8_merge_kernel<D, MODE>, dim3(ctas), 256, 0, stream, p, ctas));
+  const Decode8Launch l = decode8_launch<D, MODE>(p);
+  if (l.shared) KVB_CUDA(launch(kvb::decode8_begin_kernel, dim3(1), 1, 0, stream, static_cast<int*>(p.work)));
+  KVB_CUDA(launch(kernel, dim3(l.ctas), Cfg::kThreads, Cfg::kSmem, stream, p, maps, l.shared));
+  // few heads: the output of one goes to several blocks, of 8 quads at least
+  const int quads = p.Hq / p.Hkv * D / 4, heads = p.B * p.Hkv;
+  const int y = std::max(1, std::min(quads / 8, 4 * kvb_host::num_sms() / heads));
+  KVB_CUDA(launch(kvb::decode8_merge_kernel<D, MODE>, dim3(heads, y), kvb::D8_MERGE_THREADS, 0, stream, p, l.warps, l.shared));
   return KVSKIP_OK;
 }
 
@@ -130,10 +150,12 @@ int cache8_status(unsigned int* status) {
 
 extern "C" {
 
-int64_t kvskip_decode8_work_bytes(int G, int D) {
-  if (G < 1 || G > 16 || (D != 64 && D != 128)) return 0;
-  const int64_t cols = G <= 4 ? 4 : G <= 8 ? 8 : 16;
-  return kvb::D8_MAX_CTAS * (2 * cols * (D + 2) * static_cast<int64_t>(sizeof(float)) + 2 * static_cast<int64_t>(sizeof(int)));
+int64_t kvskip_decode8_work_bytes(const kvskip_decode8_params* p) {
+  if (!p || p->B < 1 || p->Hkv < 1 || p->Hq < p->Hkv || p->D < 1 || p->nb < 1 || (p->block_idx && p->max_blocks < 1)) return 0;
+  const int G = p->Hq / p->Hkv, mode = G <= 4 ? 0 : G <= 8 ? 1 : 2;
+  if (p->D == 128)
+    return mode == 0 ? decode8_work<128, 0>(*p) : mode == 1 ? decode8_work<128, 1>(*p) : decode8_work<128, 2>(*p);
+  return mode == 0 ? decode8_work<64, 0>(*p) : mode == 1 ? decode8_work<64, 1>(*p) : decode8_work<64, 2>(*p);
 }
 
 int kvskip_launch_decode8(const kvskip_decode8_params* p, void* stream) {

@@ -11,13 +11,13 @@
 // written back there first, which costs more than the products do.
 //
 // Work split: the (sequence, head, block) items of the whole launch are one list, ordered by sequence,
-// head and block; CTA c of C takes the items [W c / C, W (c+1) / C), its warps contiguous parts of those.
-// So requests of any mixture of lengths keep every SM busy to the end without the host knowing a length.
-// A warp keeps the running maximum, sum and output of the head it is in and has its own ring of
-// stages (a K and a V tile with an mbarrier each): no barrier between warps inside the loop.  A head that a
-// warp starts and ends is written out by that warp; the other pieces (at most two per warp) are joined in shared
-// memory in item order, and what then still is a part of a head (at most two per CTA) goes to `work` and is
-// joined by decode8_merge_kernel.  Everything is added in a fixed order: results do not depend on timing.
+// head and block, cut into chunks; a warp takes one chunk after the other.  So requests of any mixture of
+// lengths keep every SM busy to the end without the host knowing a length.  A warp keeps the running maximum, sum
+// and output of the head it is in and has its own stage (a K and a V tile with an mbarrier each, refilled as soon as
+// its products are done): no barrier between warps anywhere.  A head that a chunk holds from its first to its last
+// block is written out by the warp; other pieces (at most two per chunk) go to `work` and are joined, in item order,
+// by decode8_merge_kernel.  Where the chunks begin depends on the list alone, not on who takes them: results do not
+// depend on timing.
 //
 // P (0..1 relative to its block's maximum) goes to the tensor cores as fp16 high + low parts, which hold
 // 22 bits of it: with G <= 4 the two parts share one instruction (columns 0-3 high, 4-7 low; the scores of a
@@ -39,19 +39,53 @@ struct D8Cfg {
   static constexpr int kCols = MODE == 0 ? 4 : MODE == 1 ? 8 : 16;   // query heads there is room for
   static constexpr int kTiles = MODE == 2 ? 2 : 1;
   static constexpr int kParts = MODE == 0 ? 1 : 2;                   // MMA instructions per P fragment
-  static constexpr int kWarps = MODE == 0 ? 12 : MODE == 1 ? 10 : 8;
+  static constexpr int kWarps = MODE == 2 || D == 128 ? 8 : 12;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kStages = D == 128 ? 1 : 2;                   // per warp
   static constexpr int kTile = TILE * D;                             // bytes of a K or V tile
-  static constexpr int kRing = kWarps * kStages * 2 * kTile;
+  static constexpr int kQRow = 2 * D + 16;                           // bytes of a q row in shared memory, conflict-free
+  static constexpr int kSmem = kWarps * (2 * kTile + kCols * kQRow) + 1024;
   static constexpr int kPiece = kCols * (D + 2);                     // floats of a piece: acc, m, l
-  static constexpr int kFirst = kWarps * kPiece * 4;                 // pieces that begin before their warp's part
-  static constexpr int kSmem = kRing + kFirst + 1024;
-  static_assert(kPiece * 4 <= kStages * 2 * kTile, "a warp's last piece fits into its ring");
 };
 
 constexpr float D8_PSCALE = 13.f;   // log2 of the scaling of P
-constexpr int D8_MAX_CTAS = 160;    // bound on the grid that `work` is sized for (148 SMs)
+
+// The chunks of the work list.  Every warp has one chunk to begin with.  Under a saturated memory SMs differ by up to a
+// third in the bandwidth they get (by their place on the die), so with enough items per warp the first chunks are five
+// eighths of the list only; two eighths are cut into one more chunk per warp and the last eighth into two, which
+// the warps take from a counter as they get there.
+constexpr int D8_SHARE_MIN = 24;     // items per warp from which on chunks are taken from the counter
+struct D8Zone {                      // items from `base` on, cut into the chunks from `first` on: the first `longer` of
+  uint32_t base, first, size, longer;   // them hold size + 1, the others size
+  __device__ __forceinline__ D8Zone(uint32_t base_, uint32_t items, uint32_t first_, uint32_t chunks)
+      : base(base_), first(first_), size(chunks ? items / chunks : 0), longer(items - size * chunks) {}
+  __device__ __forceinline__ uint32_t edge(const uint32_t i) const { return base + size * (i - first) + min(i - first, longer); }
+  __device__ __forceinline__ uint32_t of(uint32_t x) const {
+    x -= base;
+    const uint32_t split = longer * (size + 1);
+    return first + (x < split ? x / (size + 1) : longer + (x - split) / size);
+  }
+};
+struct D8Chunks {
+  uint32_t wb, wc, na, nb, nc;       // items and chunks of the shared zones
+  D8Zone a, b, c;
+  __device__ __forceinline__ D8Chunks(const uint32_t W, const uint32_t warps, const int, const bool share)
+      : wb(share ? W / 4 : 0), wc(share ? W / 8 : 0), na(min(W, warps)), nb(min(wb / 3, warps)), nc(min(wc / 3, 2 * warps)),
+        a(0, W - wb - wc, 0, na), b(W - wb - wc, wb, na, nb), c(W - wc, wc, na + nb, nc) {}
+  __device__ __forceinline__ D8Chunks(const uint32_t W, const uint32_t warps, const bool counter)
+      : D8Chunks(W, warps, 0, counter && W / D8_SHARE_MIN >= warps) {}
+  __device__ __forceinline__ uint32_t count() const { return na + nb + nc; }
+  // items [begin, end) of chunk i
+  __device__ __forceinline__ void range(const uint32_t i, int& begin, int& end) const {
+    const D8Zone z = i < b.first ? a : i < c.first ? b : c;
+    begin = static_cast<int>(z.edge(i)), end = static_cast<int>(z.edge(i + 1));
+  }
+  __device__ __forceinline__ uint32_t of(const uint32_t x) const {
+    const D8Zone z = x < b.base ? a : x < c.base ? b : c;
+    return z.of(x);
+  }
+};
+// Layout of `work`: [0] the counter, [4..] items before every unit of the list, then the pieces (two per chunk).
+__host__ __device__ inline int64_t d8_piece_base(const int64_t units) { return (4 + units + 1 + 3) / 4 * 4; }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -67,6 +101,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ float2 unpack_f16(uint32_t x) {
   return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
+__device__ __forceinline__ void cp_async8(const uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -89,22 +127,22 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& x, uint32_t& 
 
 // One block of the work list, held by one lane.
 struct D8Item {
-  int bh, blk, page;   // sequence * Hkv + head; block; page (paged form) or sequence
-  int info;            // valid tokens | first of its head << 8 | last of its head << 9
-  int left;            // items of the head behind this one
+  int b, blk, page;    // sequence; block; page (paged form) or sequence
+  int info;            // valid tokens | first of its head << 8 | last of its head << 9 | KV head << 10
+  int pos;             // place in the head's blocks
   float ks, vs;
 };
 
 // Items of one unit of the list: a sequence (all heads, every block) or, with block lists, a (sequence, head).
 __device__ __forceinline__ int d8_len(const kvskip_decode8_params& p, int b) {
-  return p.lens ? max(0, min(p.lens[b], p.T)) : p.T;
+  return p.lens ? max(0, min(__ldcg(p.lens + b), p.T)) : p.T;
 }
 __device__ __forceinline__ int d8_count(const kvskip_decode8_params& p, int u) {
-  if (p.block_idx) return max(0, min(p.block_cnt[u], p.max_blocks));
+  if (p.block_idx) return max(0, min(__ldcg(p.block_cnt + u), p.max_blocks));
   return (d8_len(p, u) + TILE - 1) / TILE;
 }
 
-// Item x of the list; pref[t]: items before the units of thread t's share.
+// Item x of the list; pref[t]: items before the units of thread t's share (pref[THREADS]: all of them).
 template <int THREADS>
 __device__ __forceinline__ D8Item d8_item(const kvskip_decode8_params& p, const int* pref, const int per, const int x) {
   D8Item it;
@@ -113,40 +151,50 @@ __device__ __forceinline__ D8Item d8_item(const kvskip_decode8_params& p, const 
     const int mid = (lo + hi + 1) >> 1;
     if (pref[mid] <= x) lo = mid; else hi = mid - 1;
   }
+  const uint32_t Hkv = p.Hkv;
   const int mul = p.block_idx ? 1 : p.Hkv;
-  int rem = x - pref[lo], u = lo * per, cnt = d8_count(p, u);
-  while (rem >= cnt * mul) {
-    rem -= cnt * mul;
-    cnt = d8_count(p, ++u);
+  int rem = x - pref[lo], u = lo, cnt;
+  if (per == 1) {
+    cnt = pref[lo + 1] - pref[lo];
+    if (!p.block_idx) cnt = static_cast<int>(static_cast<uint32_t>(cnt) / Hkv);
+  } else {
+    u = lo * per, cnt = d8_count(p, u);
+    while (rem >= cnt * mul) {
+      rem -= cnt * mul;
+      cnt = d8_count(p, ++u);
+    }
   }
   int b, h, j;
   if (p.block_idx) {
-    b = u / p.Hkv, h = u - b * p.Hkv, j = rem;
+    b = static_cast<int>(static_cast<uint32_t>(u) / Hkv), h = u - b * p.Hkv, j = rem;
     it.blk = p.block_idx[static_cast<int64_t>(u) * p.max_blocks + j];
   } else {
-    b = u, h = rem / cnt, j = rem - h * cnt;
+    b = u, h = static_cast<int>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(cnt)), j = rem - h * cnt;
     it.blk = j;
   }
-  it.bh = b * p.Hkv + h;
+  it.b = b;
   const bool in = it.blk >= 0 && it.blk < p.nb;
   const int tok = in ? max(0, min(TILE, d8_len(p, b) - it.blk * TILE)) : 0;
-  it.info = tok | (j == 0 ? 256 : 0) | (j == cnt - 1 ? 512 : 0);
-  it.left = cnt - 1 - j;
+  it.info = tok | (j == 0 ? 256 : 0) | (j == cnt - 1 ? 512 : 0) | (h << 10);
+  it.pos = j;
   it.ks = it.vs = 0.f;
   it.page = b;
+  // (a listed block behind the length has no scale: what is there may be anything.  Nothing here uses the
+  // scales once they are asked for, so that the loads of the first block need not wait for them.)
   if (p.page_table) {
     it.page = in ? p.page_table[static_cast<int64_t>(b) * p.max_pages + it.blk] : -1;
     if (it.page >= 0 && it.page < p.num_pages) {
-      it.ks = p.k_scale[it.page * p.ks_sb + h * p.ks_sh];
-      it.vs = p.v_scale[it.page * p.vs_sb + h * p.vs_sh];
+      if (tok > 0) {
+        it.ks = p.k_scale[it.page * p.ks_sb + h * p.ks_sh];
+        it.vs = p.v_scale[it.page * p.vs_sb + h * p.vs_sh];
+      }
     } else {
       it.page = -1;                      // out of bounds for the tensor map: reads as zeros
     }
-  } else if (in) {
+  } else if (tok > 0) {
     it.ks = p.k_scale[b * p.ks_sb + h * p.ks_sh + it.blk * p.ks_st];
     it.vs = p.v_scale[b * p.vs_sb + h * p.vs_sh + it.blk * p.vs_st];
   }
-  if (tok == 0) it.ks = it.vs = 0.f;     // a listed block behind the length: its scale may be anything
   return it;
 }
 
@@ -158,39 +206,55 @@ __device__ __forceinline__ void d8_store(const kvskip_decode8_params& p, const i
   *reinterpret_cast<uint32_t*>(p.out + hq * p.D + d0) = w;
   if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + hq * p.D + d0) = make_float2(a, b);
 }
+// four channels of a row that is divided by its sum
+__device__ __forceinline__ void d8_store4(const kvskip_decode8_params& p, const int64_t hq, const int d0, float4 x, const float l) {
+  if (l == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
+  else x.x /= l, x.y /= l, x.z /= l, x.w /= l;
+  d8_store(p, hq, d0, x.x, x.y);
+  d8_store(p, hq, d0 + 2, x.z, x.w);
+}
 __device__ __forceinline__ float d8_lse(float m, float l) {
   return l == 0.f ? -INFINITY : (m + log2f(l) - D8_PSCALE) * LN2;   // (a NaN sum stays one)
 }
 __device__ __forceinline__ float d8_safe(float m) { return m == -INFINITY ? 0.f : m; }
 
+// Zeroes the counter of a launch whose warps share chunks.
+__global__ void decode8_begin_kernel(int* counter) {
+  pdl_wait_prior();
+  pdl_launch_dependents();
+  *counter = 0;
+}
+
 template <int KIND, int D, int MODE>
 __global__ void __launch_bounds__(D8Cfg<D, MODE>::kThreads, 1)
-decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_constant__ D8Maps maps, const int min_items) {
+decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_constant__ D8Maps maps, const int shared) {
   using Cfg = D8Cfg<D, MODE>;
-  constexpr int NW = Cfg::kWarps, NT = Cfg::kThreads, ST = Cfg::kStages, KS = D / 16;
+  constexpr int NW = Cfg::kWarps, NT = Cfg::kThreads, KS = D / 16;
   constexpr int CT = Cfg::kTiles, PT = Cfg::kParts, COLS = Cfg::kCols;
 
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t bars[NW * ST * 2];
-  __shared__ int pref[NT];
+  __shared__ uint64_t bars[NW * 2];
+  __shared__ int pref[NT + 1];
   __shared__ int wsum[NW];
-  __shared__ int piece_bh[2 * NW], piece_flag[2 * NW], piece_end[2 * NW];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int c = blockIdx.x;
   const int G = p.Hq / p.Hkv;
   const int g = lane >> 2, q4 = lane & 3;
   if (tid == 0) {
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.v);
   }
-  if (tid < NW * ST * 2) mbar_init(&bars[tid], 1);
-  if (tid < 2 * NW) piece_bh[tid] = -1;
+  if (tid < NW * 2) mbar_init(&bars[tid], 1);
   mbar_fence_init();
   pdl_wait_prior();
   pdl_launch_dependents();
 
+  if (p.page_table) {
+    // the page table into L2 while the lengths are on their way (128 bytes a thread cover 7 MB of it)
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * NT + tid) * 32;
+    if (at < static_cast<int64_t>(p.B) * p.max_pages) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.page_table + at));
+  }
   // ---- the work list: items before every thread's share of the units, and all of them
   const int units = p.block_idx ? p.B * p.Hkv : p.B;
   const int mul = p.block_idx ? 1 : p.Hkv;
@@ -212,130 +276,150 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
     W += wsum[w];
   }
   pref[tid] = before + incl - mine;
+  if (tid == 0) pref[NT] = W;
   __syncthreads();
 
-  const int C = max(1, min(static_cast<int>(gridDim.x), (W + min_items - 1) / min_items));
-  float* work = static_cast<float*>(p.work);
-  int* meta = reinterpret_cast<int*>(work + 2 * static_cast<int64_t>(gridDim.x) * Cfg::kPiece);
-  const int c0 = c < C ? static_cast<int>(static_cast<int64_t>(W) * c / C) : 0;
-  const int c1 = c < C ? static_cast<int>(static_cast<int64_t>(W) * (c + 1) / C) : 0;
-  const int w0 = c0 + static_cast<int>(static_cast<int64_t>(c1 - c0) * warp / NW);
-  const int n = c0 + static_cast<int>(static_cast<int64_t>(c1 - c0) * (warp + 1) / NW) - w0;
+  int* counter = static_cast<int*>(p.work);
+  float* pieces = static_cast<float*>(p.work) + d8_piece_base(units);
+  const D8Chunks cut(W, NW * gridDim.x, shared);
+  if (blockIdx.x == 0) {                 // for the join: items before every unit
+    int x = pref[tid];
+    for (int u = tid * per; u < min(units, (tid + 1) * per); ++u) {
+      counter[4 + u] = x;
+      if (per > 1) x += d8_count(p, u) * mul;
+    }
+    if (tid == 0) counter[4 + units] = W;
+  }
 
-  float* first_piece = reinterpret_cast<float*>(smem + Cfg::kRing) + warp * Cfg::kPiece;
-  float* last_piece = reinterpret_cast<float*>(smem + warp * ST * 2 * Cfg::kTile);   // on top of the warp's ring
+  // neighbouring chunks on different SMs: a short list spreads over all of them
+  int chunk = warp * gridDim.x + blockIdx.x;
+  int begin = 0, end = 0;                // what is left of the chunk
+  if (static_cast<uint32_t>(chunk) < cut.na) cut.range(chunk, begin, end);
 
-  if (n > 0) {
-    unsigned char* ring = smem + warp * ST * 2 * Cfg::kTile;
-    uint64_t* bar = bars + warp * ST * 2;      // [stage][K, V]
-    // items 32 i .. 32 i + 31 of this warp are in the lanes of `now`, the 32 behind them in `next`
-    D8Item now = d8_item<NT>(p, pref, per, w0 + min(lane, n - 1));
-    D8Item next = now;
+  if (begin < end) {
+    unsigned char* kstage = smem + warp * 2 * Cfg::kTile;
+    unsigned char* vstage = kstage + Cfg::kTile;
+    unsigned char* qstage = smem + NW * 2 * Cfg::kTile + warp * COLS * Cfg::kQRow;
+    uint64_t* bar = bars + 2 * warp;     // K, V
+    int phase = 0;
+    // up to 32 items of a chunk are in the lanes of `now`, the ones behind them (of the next chunk, at its end) in `next`
+    int n = min(32, end - begin);
+    int next_n = 0, next_begin = 0, next_end = end, next_chunk = chunk;
+    D8Item now = d8_item<NT>(p, pref, per, begin + min(lane, n - 1)), next = now;
 
-    auto load = [&](const int i, const int base, const bool is_v) {   // item i -> its stage
-      const bool far = (i >> 5) != base;
-      const int bh = __shfl_sync(0xffffffffu, far ? next.bh : now.bh, i & 31);
-      const int blk = __shfl_sync(0xffffffffu, far ? next.blk : now.blk, i & 31);
-      const int page = __shfl_sync(0xffffffffu, far ? next.page : now.page, i & 31);
+    int64_t cur = -1;                    // first row of q of the head the warp is in
+    auto load = [&](const D8Item& from, const int i, const bool is_v) {
+      const int h = __shfl_sync(0xffffffffu, from.info, i) >> 10;
+      const int blk = __shfl_sync(0xffffffffu, from.blk, i);
+      const int page = __shfl_sync(0xffffffffu, from.page, i);
       if (lane == 0) {
-        const int s = i % ST;
-        uint64_t* b = &bar[2 * s + is_v];
-        mbar_expect_tx(b, Cfg::kTile);
-        tma_load_4d(ring + (2 * s + is_v) * Cfg::kTile, is_v ? &maps.v : &maps.k, b, 0, p.page_table ? 0 : blk * TILE,
-                    bh % p.Hkv, page);
+        mbar_expect_tx(&bar[is_v], Cfg::kTile);
+        tma_load_4d(is_v ? vstage : kstage, is_v ? &maps.v : &maps.k, &bar[is_v], 0, p.page_table ? 0 : blk * TILE,
+                    h, page);
+      }
+      if (!is_v) {                       // another head: its rows of q come along
+        const int b = __shfl_sync(0xffffffffu, from.b, i);
+        if (static_cast<int64_t>(b) * p.Hq + h * G != cur) {
+          const uint16_t* src = p.q + b * p.q_sb + static_cast<int64_t>(h) * G * p.q_sh;
+          for (int o = lane; o < G * (D / 4); o += 32)
+            cp_async8(smem_u32(qstage + o / (D / 4) * Cfg::kQRow + o % (D / 4) * 8), src + o / (D / 4) * p.q_sh + o % (D / 4) * 4);
+        }
       }
     };
-#pragma unroll
-    for (int i = 0; i < ST; ++i)
-      if (i < n) {
-        load(i, 0, false);
-        load(i, 0, true);
-      }
-    if (n > 32) next = d8_item<NT>(p, pref, per, w0 + min(32 + lane, n - 1));
+    load(now, 0, false);
+    load(now, 0, true);
 
     uint32_t bq[CT][KS][2];
     float cm[CT][2];                       // softmax scale / row scale of q of this thread's two columns
     float m_run[CT][2], l_run[CT][2], acc[KS][CT][4];
-    int cur = -1, began = 0;
+    int began = 0;
 
     // the piece of head `cur`: written out if it is the whole head, else kept for the join
-    auto flush = [&](const bool ends, const int end_item) {
+    auto flush = [&](const bool ends) {
       float l[CT][2];
 #pragma unroll
       for (int t = 0; t < CT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) l[t][e] = quadcol_sum(l_run[t][e]);
-      const int64_t hq0 = static_cast<int64_t>(cur / p.Hkv) * p.Hq + (cur % p.Hkv) * G;
+      const int64_t hq0 = cur;
       if (MODE == 0) {
 #pragma unroll
         for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[mt][0][i] += __shfl_xor_sync(0xffffffffu, acc[mt][0][i], 2);
+        if (q4 >= 2) return;             // (the columns of the low parts: their sums are in the other half)
       }
-      float* dst = began ? last_piece : first_piece;
-      if (MODE == 0 && q4 >= 2) {
-        // (the columns of the low parts: their sums are in the other half)
-      } else {
+      float* dst = pieces + (2 * static_cast<int64_t>(chunk) + began) * Cfg::kPiece;
 #pragma unroll
-        for (int t = 0; t < CT; ++t)
+      for (int t = 0; t < CT; ++t)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int head = 8 * t + 2 * q4 + e;
-            if (head >= G) continue;
-            if (began && ends) {
-              const float inv = l[t][e] == 0.f ? 0.f : __fdividef(1.f, l[t][e]);
+        for (int e = 0; e < 2; ++e) {
+          const int head = 8 * t + 2 * q4 + e;
+          if (head >= G) continue;
+          if (began && ends) {
+            const bool none = l[t][e] == 0.f;
+            const float inv = none ? 0.f : __fdividef(1.f, l[t][e]);
 #pragma unroll
-              for (int mt = 0; mt < KS; ++mt) {
-                const float a = l[t][e] == 0.f ? 0.f : acc[mt][t][e] * inv, b = l[t][e] == 0.f ? 0.f : acc[mt][t][e + 2] * inv;
-                d8_store(p, hq0 + head, mt * 16 + 2 * g, a, b);
-              }
-              if (g == 0) p.lse[hq0 + head] = d8_lse(m_run[t][e], l[t][e]);
-            } else {
+            for (int mt = 0; mt < KS; ++mt)
+              d8_store(p, hq0 + head, mt * 16 + 2 * g, none ? 0.f : acc[mt][t][e] * inv, none ? 0.f : acc[mt][t][e + 2] * inv);
+            if (g == 0) p.lse[hq0 + head] = d8_lse(m_run[t][e], l[t][e]);
+          } else {
 #pragma unroll
-              for (int mt = 0; mt < KS; ++mt)
-                *reinterpret_cast<float2*>(dst + head * D + mt * 16 + 2 * g) = make_float2(acc[mt][t][e], acc[mt][t][e + 2]);
-              if (g == 0) {
-                dst[COLS * D + head] = m_run[t][e];
-                dst[COLS * D + COLS + head] = l[t][e];
-              }
+            for (int mt = 0; mt < KS; ++mt)
+              *reinterpret_cast<float2*>(dst + head * D + mt * 16 + 2 * g) = make_float2(acc[mt][t][e], acc[mt][t][e + 2]);
+            if (g == 0) {
+              dst[COLS * D + head] = m_run[t][e];
+              dst[COLS * D + COLS + head] = l[t][e];
             }
           }
-      }
-      if (!(began && ends) && lane == 0) {
-        piece_bh[2 * warp + began] = cur;
-        piece_flag[2 * warp + began] = began | (ends ? 2 : 0);
-        piece_end[2 * warp + began] = end_item;
-      }
+        }
     };
 
-    for (int i = 0; i < n; ++i) {
-      const int li = i & 31, base = i >> 5;
-      if (li == 0 && i > 0) {
-        now = next;
-        if (i + 32 < n) next = d8_item<NT>(p, pref, per, w0 + min(i + 32 + lane, n - 1));
+    int li = 0, taken = 0;
+    for (;;) {
+      const bool tail = begin + n == end;          // these are the chunk's last items
+      if (li == 0 && !tail) {
+        next_begin = begin + n;
+        next_n = min(32, end - next_begin);
+        next = d8_item<NT>(p, pref, per, next_begin + min(lane, next_n - 1));
       }
-      const int bh = __shfl_sync(0xffffffffu, now.bh, li);
+      if (tail && cut.nb) {                        // take a chunk, one item ahead of its first load
+        if (li == max(0, n - 2) && lane == 0) taken = atomicAdd(counter, 1);
+        if (li == n - 1) {
+          const uint32_t got = cut.na + __shfl_sync(0xffffffffu, taken, 0);
+          if (got < cut.count()) {
+            next_chunk = static_cast<int>(got);
+            cut.range(got, next_begin, next_end);
+            next_n = min(32, next_end - next_begin);
+            next = d8_item<NT>(p, pref, per, next_begin + min(lane, next_n - 1));
+          }
+        }
+      }
+      const bool last = li == n - 1;
+      const int b = __shfl_sync(0xffffffffu, now.b, li);
       const int blk = __shfl_sync(0xffffffffu, now.blk, li);
       const int info = __shfl_sync(0xffffffffu, now.info, li);
-      const int left = __shfl_sync(0xffffffffu, now.left, li);
+      const int pos = __shfl_sync(0xffffffffu, now.pos, li);
       const float ks = __shfl_sync(0xffffffffu, now.ks, li);
       const float vs = __shfl_sync(0xffffffffu, now.vs, li);
-      const int b = bh / p.Hkv, h = bh - b * p.Hkv, tok = info & 255;
+      const int h = info >> 10, tok = info & 255;
       const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + h * G;
 
-      if (bh != cur) {
-        cur = bh;
+      if (hq0 != cur) {
+        cur = hq0;
         began = (info >> 8) & 1;
         // Q^T as the B operand: column n = lane / 4; row k = 2 c, 2 c + 1 (+8) of a 16-step is channel
         // 4 c + 0..3 of it, the order in which ldmatrix hands a lane the codes of a K row
         float inv[CT];
+        cp_async_wait();
+        __syncwarp();
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
           const int head = MODE == 0 ? (g & 3) : 8 * t + g;
           uint2 w[KS];
-          const uint16_t* qp = p.q + b * p.q_sb + (static_cast<int64_t>(h) * G + min(head, G - 1)) * p.q_sh + 4 * q4;
+          const unsigned char* qp = qstage + min(head, G - 1) * Cfg::kQRow + 8 * q4;
 #pragma unroll
-          for (int s = 0; s < KS; ++s) w[s] = *reinterpret_cast<const uint2*>(qp + 16 * s);
+          for (int s = 0; s < KS; ++s) w[s] = *reinterpret_cast<const uint2*>(qp + 32 * s);
           float x[KS][4], top = 0.f;
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
@@ -376,7 +460,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
         // statistics of blocks that are not read: up to the previous item of the head, and behind its last one
         int prev = blk - 1, stop = blk;
         if (p.block_idx)
-          prev = (info & 256) ? -1 : p.block_idx[static_cast<int64_t>(bh) * p.max_blocks + d8_count(p, bh) - left - 2];
+          prev = (info & 256) ? -1 : p.block_idx[(static_cast<int64_t>(b) * p.Hkv + h) * p.max_blocks + pos - 1];
         if (info & 512) stop = p.nb;
         for (int x = max(0, prev + 1) + lane; x < min(stop, p.nb); x += 32)
           if (x != blk)
@@ -386,8 +470,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
             }
       }
 
-      const int s = i % ST;
-      const uint32_t kt = smem_u32(ring + 2 * s * Cfg::kTile), vt = kt + Cfg::kTile;
+      const uint32_t kt = smem_u32(kstage), vt = kt + Cfg::kTile;
       // 16-byte chunk `ch` of row r: the tiles are swizzled over 128 bytes (D = 128) or 64 (D = 64)
       auto at = [&](const uint32_t tile, const int r, const int ch) -> uint32_t {
         if constexpr (D == 128) return tile + r * 128 + ((ch ^ (r & 7)) << 4);
@@ -395,7 +478,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
       };
       const int lrow = lane & 7, lmat = lane >> 3;
 
-      if (!mbar_wait(&bar[2 * s], (i / ST) & 1, 0x600u + warp)) break;
+      if (!mbar_wait(&bar[0], phase, 0x600u + warp)) break;
       // ---- S^T = K Q^T: 4 tiles of 16 tokens x 8 columns
       float sc[CT][4][4];
 #pragma unroll
@@ -421,7 +504,8 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
         }
       }
       __syncwarp();
-      if (i + ST < n) load(i + ST, base, false);
+      if (!last) load(now, li + 1, false);
+      else if (next_n > 0) load(next, 0, false);
 
       // ---- softmax relative to the block's own maximum, joined with the running one
       uint32_t pb[CT][4][PT][2];
@@ -496,13 +580,15 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
         }
       }
 
-      if (!mbar_wait(&bar[2 * s + 1], (i / ST) & 1, 0x620u + warp)) break;
-      if (tok < TILE) {
-        // V rows behind the length: their weights are zero, but zero times a NaN code is not
-        unsigned char* vrow = ring + (2 * s + 1) * Cfg::kTile;
-        for (int o = tok * D + lane * 16; o < TILE * D; o += 512) *reinterpret_cast<uint4*>(vrow + o) = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async_smem();          // ordered before the next load into this stage
-        __syncwarp();
+      if (!mbar_wait(&bar[1], phase, 0x620u + warp)) break;
+      // V rows behind the length: their weights are zero, but zero times a NaN code is not (int8 has none)
+      uint32_t vmask[8];
+      if constexpr (KIND == KVSKIP_KIND_E4M3) {
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          const int t = m * 8 + 2 * q4;          // a register of the fragment holds two codes of tokens t and t + 1 each
+          vmask[m] = t + 1 < tok ? 0xffffffffu : t < tok ? 0xffffu : 0u;
+        }
       }
       // ---- O^T = alpha O^T + beta vs V^T P^T: row g of a tile is channel 2 g, row g + 8 channel 2 g + 1
       // (two adjacent codes of a token travel as one 16-bit unit through the transposing ldmatrix)
@@ -518,6 +604,10 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
         for (int th = 0; th < 2; ++th) {
           uint32_t r[4];
           ldsm_x4_t(r, at(vt, th * 32 + lmat * 8 + lrow, mt));
+          if constexpr (KIND == KVSKIP_KIND_E4M3) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) r[m] &= vmask[th * 4 + m];
+          }
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
             uint32_t a[4];
@@ -538,120 +628,147 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
           }
       }
       __syncwarp();
-      if (i + ST < n) load(i + ST, base, true);
+      if (!last) load(now, li + 1, true);
+      else if (next_n > 0) load(next, 0, true);
+      phase ^= 1;
 
       const bool ends = (info >> 9) & 1;
-      if (ends || i + 1 == n) flush(ends, w0 + i + left);
+      if (ends || (last && tail)) flush(ends);
       if (ends) cur = -1;
-    }
-  }
-
-  // ---- heads without an item: zeros
-  for (int bh = c * NW + warp; bh < p.B * p.Hkv; bh += gridDim.x * NW) {
-    if (d8_count(p, p.block_idx ? bh : bh / p.Hkv) > 0) continue;
-    const int64_t hq0 = static_cast<int64_t>(bh / p.Hkv) * p.Hq + (bh % p.Hkv) * G;
-    for (int o = lane; o < G * D / 2; o += 32) d8_store(p, hq0 + o / (D / 2), 2 * (o % (D / 2)), 0.f, 0.f);
-    if (lane < G) p.lse[hq0 + lane] = -INFINITY;
-    if (p.blk_max)
-      for (int o = lane; o < G * p.nb; o += 32) {
-        p.blk_max[hq0 * p.nb + o] = -INFINITY;
-        p.blk_sum[hq0 * p.nb + o] = 0.f;
+      if (!last) {
+        ++li;
+        continue;
       }
-  }
-  __syncthreads();
-
-  // ---- join of the warps' pieces, in item order
-  int next_bh = -1, next_ctas = 0;       // head that goes on in the next CTA
-  for (int a = 0; a < 2 * NW;) {
-    const int bh = piece_bh[a];
-    if (bh < 0) {
-      ++a;
-      continue;
+      if (next_n == 0) break;
+      now = next;
+      li = 0, n = next_n, next_n = 0;
+      begin = next_begin, end = next_end, chunk = next_chunk;
     }
-    int z = a, lastp = a;                // pieces a..lastp belong to the head
-    while (++z < 2 * NW) {
-      if (piece_bh[z] < 0) continue;
-      if (piece_bh[z] != bh) break;
-      lastp = z;
-    }
-    const bool begins = piece_flag[a] & 1, ends = piece_flag[lastp] & 2;
-    const int64_t hq0 = static_cast<int64_t>(bh / p.Hkv) * p.Hq + (bh % p.Hkv) * G;
-    float* out_piece = work + (2 * static_cast<int64_t>(c) + begins) * Cfg::kPiece;
-    for (int o = tid; o < G * D / 2; o += NT) {
-      const int head = o / (D / 2), d0 = 2 * (o % (D / 2));
-      float m = -INFINITY;
-      for (int y = a; y <= lastp; ++y) {
-        if (piece_bh[y] < 0) continue;
-        const float* src = (y & 1) ? reinterpret_cast<float*>(smem + (y >> 1) * ST * 2 * Cfg::kTile)
-                                   : reinterpret_cast<float*>(smem + Cfg::kRing) + (y >> 1) * Cfg::kPiece;
-        m = fmaxf(m, src[COLS * D + head]);
-      }
-      const float mu = d8_safe(m);
-      float l = 0.f, x0 = 0.f, x1 = 0.f;
-      for (int y = a; y <= lastp; ++y) {
-        if (piece_bh[y] < 0) continue;
-        const float* src = (y & 1) ? reinterpret_cast<float*>(smem + (y >> 1) * ST * 2 * Cfg::kTile)
-                                   : reinterpret_cast<float*>(smem + Cfg::kRing) + (y >> 1) * Cfg::kPiece;
-        const float w = ex2(src[COLS * D + head] - mu);
-        const float2 v = *reinterpret_cast<const float2*>(src + head * D + d0);
-        l += src[COLS * D + COLS + head] * w;
-        x0 += v.x * w;
-        x1 += v.y * w;
-      }
-      if (begins && ends) {
-        d8_store(p, hq0 + head, d0, l == 0.f ? 0.f : x0 / l, l == 0.f ? 0.f : x1 / l);
-        if (d0 == 0) p.lse[hq0 + head] = d8_lse(m, l);
-      } else {
-        *reinterpret_cast<float2*>(out_piece + head * D + d0) = make_float2(x0, x1);
-        if (d0 == 0) {
-          out_piece[COLS * D + head] = m;
-          out_piece[COLS * D + COLS + head] = l;
-        }
-      }
-    }
-    if (begins && !ends) {
-      // the CTA that holds item x is the last c' with floor(W c' / C) <= x
-      next_bh = bh;
-      next_ctas = static_cast<int>(((static_cast<int64_t>(piece_end[lastp]) + 1) * C - 1) / W) - c;
-    }
-    a = z;
-  }
-  if (tid == 0) {
-    meta[2 * c] = next_bh;
-    meta[2 * c + 1] = next_ctas;
   }
 }
 
-// Heads that are spread over several CTAs: block c joins the head that begins in CTA c and goes on behind it.
+// The join: block (bh, y) does its share of the output of KV head bh, if the head's items lie in more than one chunk, or
+// writes the zeros of a head without items.  A thread has four channels of a query head (a quad) and every S-th piece,
+// eight pieces in flight; the S sums are added in order.
+constexpr int D8_MERGE_THREADS = 256;
 template <int D, int MODE>
-__global__ void __launch_bounds__(256) decode8_merge_kernel(const __grid_constant__ kvskip_decode8_params p, const int ctas) {
+__global__ void __launch_bounds__(D8_MERGE_THREADS)
+decode8_merge_kernel(const __grid_constant__ kvskip_decode8_params p, const int warps, const int shared) {
   using Cfg = D8Cfg<D, MODE>;
-  constexpr int COLS = Cfg::kCols;
+  constexpr int COLS = Cfg::kCols, L = D / 4, NT = D8_MERGE_THREADS;
+  __shared__ float4 sx[NT];
+  __shared__ float sl[NT], sm[NT];
+  __shared__ int wsum[NT / 32], span[2];
+  const int bh = blockIdx.x, G = p.Hq / p.Hkv, tid = threadIdx.x, lane = tid & 31;
+  const int units = p.block_idx ? p.B * p.Hkv : p.B;
+  const int* pref = static_cast<const int*>(p.work) + 4;
+  const int b = bh / p.Hkv, u = p.block_idx ? bh : b;
+  int first, count, W;
+  if (units <= NT) {
+    // Before the wait: the lengths are older than the kernel this one waits for (which let this one begin only after
+    // its own wait), so the place of the head in the list can be had while that one is at work.
+    const int mine = tid < units ? d8_count(p, tid) * (p.block_idx ? 1 : p.Hkv) : 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) wsum[tid >> 5] = incl;
+    __syncthreads();
+    W = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w < (tid >> 5)) incl += wsum[w];
+      W += wsum[w];
+    }
+    if (tid == u) span[0] = incl - mine, span[1] = mine;
+    __syncthreads();
+    first = span[0], count = span[1];
+  } else {
+    pdl_wait_prior();
+    first = pref[u], count = pref[u + 1] - first, W = pref[units];
+  }
+  if (!p.block_idx) {
+    count = static_cast<int>(static_cast<uint32_t>(count) / static_cast<uint32_t>(p.Hkv));
+    first += (bh - b * p.Hkv) * count;
+  }
+  const D8Chunks cut(W, warps, shared);
+  int c0 = 0, c1 = 0;
+  if (count) c0 = static_cast<int>(cut.of(first)), c1 = static_cast<int>(cut.of(first + count - 1));
   pdl_wait_prior();
   pdl_launch_dependents();
-  const int c = blockIdx.x, G = p.Hq / p.Hkv;
-  const float* work = static_cast<const float*>(p.work);
-  const int* meta = reinterpret_cast<const int*>(work + 2 * static_cast<int64_t>(ctas) * Cfg::kPiece);
-  const int bh = meta[2 * c], more = meta[2 * c + 1];
-  if (bh < 0) return;
-  const int64_t hq0 = static_cast<int64_t>(bh / p.Hkv) * p.Hq + (bh % p.Hkv) * G;
-  auto piece = [&](int y) { return work + (2 * static_cast<int64_t>(c + y) + (y == 0 ? 1 : 0)) * Cfg::kPiece; };
-  for (int o = threadIdx.x; o < G * D / 2; o += blockDim.x) {
-    const int head = o / (D / 2), d0 = 2 * (o % (D / 2));
-    float m = -INFINITY;
-    for (int y = 0; y <= more; ++y) m = fmaxf(m, piece(y)[COLS * D + head]);
-    const float mu = d8_safe(m);
-    float l = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int y = 0; y <= more; ++y) {
-      const float* src = piece(y);
-      const float w = ex2(src[COLS * D + head] - mu);
-      const float2 v = *reinterpret_cast<const float2*>(src + head * D + d0);
-      l += src[COLS * D + COLS + head] * w;
-      x0 += v.x * w;
-      x1 += v.y * w;
+  const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + (bh - b * p.Hkv) * G;
+  const int quad0 = G * L * blockIdx.y / gridDim.y, quads = G * L * (blockIdx.y + 1) / gridDim.y - quad0;
+  if (count == 0) {
+    for (int o = tid; o < quads; o += NT) d8_store4(p, hq0 + (quad0 + o) / L, 4 * ((quad0 + o) % L), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+    if (blockIdx.y) return;
+    if (tid < G) p.lse[hq0 + tid] = -INFINITY;
+    if (p.blk_max)
+      for (int64_t o = tid; o < static_cast<int64_t>(G) * p.nb; o += NT) {
+        p.blk_max[hq0 * p.nb + o] = -INFINITY;
+        p.blk_sum[hq0 * p.nb + o] = 0.f;
+      }
+    return;
+  }
+  if (c0 == c1) return;                  // written by the warp that had it
+  // the first piece begins the head, the others go on from a chunk's beginning
+  const float* pieces = static_cast<const float*>(p.work) + d8_piece_base(units);
+  const int S = quads >= NT ? 1 : min(NT / quads, (c1 - c0 + 8) / 8);
+  for (int q0 = 0; q0 < quads; q0 += NT) {
+    const int s = S == 1 ? 0 : tid / quads, at = S == 1 ? q0 + tid : tid - s * quads;
+    const bool on = s < S && at < quads;
+    const int quad = quad0 + at, head = quad / L, d0 = 4 * (quad % L);
+    float m = -INFINITY, l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = c0 + s; on && c <= c1; c += 8 * S) {
+      float pm[8], pl[8];
+      float4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int y = min(c + i * S, c1);
+        const float* src = pieces + (2 * static_cast<int64_t>(y) + (y == c0 ? 1 : 0)) * Cfg::kPiece;
+        pm[i] = src[COLS * D + head];
+        pl[i] = src[COLS * D + COLS + head];
+        v[i] = *reinterpret_cast<const float4*>(src + head * D + d0);
+      }
+      const float m_old = m;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (c + i * S > c1) pm[i] = -INFINITY, pl[i] = 0.f, v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        m = fmaxf(m, pm[i]);
+      }
+      const float mu = d8_safe(m), down = ex2(m_old - mu);
+      l *= down;
+      x.x *= down, x.y *= down, x.z *= down, x.w *= down;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = ex2(pm[i] - mu);
+        l += pl[i] * f;
+        x.x += v[i].x * f, x.y += v[i].y * f, x.z += v[i].z * f, x.w += v[i].w * f;
+      }
     }
-    d8_store(p, hq0 + head, d0, l == 0.f ? 0.f : x0 / l, l == 0.f ? 0.f : x1 / l);
-    if (d0 == 0) p.lse[hq0 + head] = d8_lse(m, l);
+    if (S > 1) {
+      sx[tid] = x, sl[tid] = l, sm[tid] = m;
+      __syncthreads();
+      if (s == 0 && on) {
+#pragma unroll 8
+        for (int i = 1; i < S; ++i) m = fmaxf(m, sm[i * quads + at]);
+        const float mu = d8_safe(m);
+        l = 0.f, x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (int i = 0; i < S; ++i) {
+          const float f = ex2(sm[i * quads + at] - mu);
+          const float4 v = sx[i * quads + at];
+          l += sl[i * quads + at] * f;
+          x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
+        }
+      }
+    }
+    if (s == 0 && on) {
+      d8_store4(p, hq0 + head, d0, x, l);
+      if (d0 == 0) p.lse[hq0 + head] = d8_lse(m, l);
+    }
   }
 }
 

@@ -804,8 +804,6 @@ std::vector<at::Tensor> decode8(const at::Tensor& q, const at::Tensor& k, const 
     p.blk_max = bmax.data_ptr<float>();
     p.blk_sum = bsum.data_ptr<float>();
   }
-  const int G = static_cast<int>(Hq / Hkv);
-  at::Tensor work = at::empty({kvskip_decode8_work_bytes(G, static_cast<int>(D))}, q.options().dtype(at::kByte));
   p.q = u16(q);
   p.q_sb = q.stride(0); p.q_sh = q.stride(1);
   p.k = u8(k); p.v = u8(v);
@@ -824,6 +822,7 @@ std::vector<at::Tensor> decode8(const at::Tensor& q, const at::Tensor& k, const 
   p.out = u16m(out);
   if (want_f32) p.out_f32 = out32.data_ptr<float>();
   p.lse = lse.data_ptr<float>();
+  const at::Tensor work = at::empty({kvskip_decode8_work_bytes(&p)}, q.options().dtype(at::kByte));
   p.work = work.data_ptr();
   raise_on(kvskip_launch_decode8(&p, cur_stream()));
   return {out, lse, bmax, bsum, out32};

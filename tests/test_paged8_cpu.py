@@ -68,8 +68,9 @@ def test_decode8_entry_refuses(lib, change, text):
 def test_null_blocks_and_sizes(lib):
     for n in ("decode8", "write8", "extend_pages", "release_pages"):
         assert getattr(lib, f"kvskip_launch_{n}")(None, None) == -1 and b"null" in lib.kvskip_last_error()
-    assert lib.kvskip_decode8_work_bytes(17, 128) == 0 and lib.kvskip_decode8_work_bytes(4, 96) == 0
-    assert lib.kvskip_decode8_work_bytes(16, 128) > lib.kvskip_decode8_work_bytes(4, 128) > 0
+    size = lambda **kw: lib.kvskip_decode8_work_bytes(ctypes.byref(_decode_params(**kw)))  # noqa: E731
+    assert size(B=0) == 0 and size(nb=0) == 0 and size(block_idx=4096) == 0
+    assert size(Hq=128) > size() > 0 and size(nb=4000) > size()
 
 
 @pytest.mark.parametrize("change,text", [
