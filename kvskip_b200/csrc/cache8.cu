@@ -109,15 +109,24 @@ int by_group(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cudaStream
   return launch_decode8<KIND, D, 2>(p, maps, s);
 }
 
-template <int KIND, int D>
+template <int KIND, int D, bool F16>
 int by_chunk(const kvskip_write8_params& p, cudaStream_t s) {
   // The slots of a CTA: 64 when that still gives every SM work, else 8, so that the tokens of a decode step
-  // spread over the GPU.
-  if ((p.n + 63) / 64 * p.Hkv * 2 >= 2 * static_cast<int64_t>(kvb_host::num_sms()))
-    KVB_CUDA(launch(kvb::write8_kernel<KIND, D, 64>, dim3(static_cast<unsigned>((p.n + 63) / 64), p.Hkv, 2), kvb::W8_THREADS, 0, s, p));
-  else
-    KVB_CUDA(launch(kvb::write8_kernel<KIND, D, 8>, dim3(static_cast<unsigned>((p.n + 7) / 8), p.Hkv, 2), kvb::W8_THREADS, 0, s, p));
+  // spread over the GPU.  Pairs of a CTA: as many as leave 16 CTAs per SM.
+  const int64_t sms = kvb_host::num_sms(), pairs = 2 * static_cast<int64_t>(p.Hkv), chunks = (p.n + 63) / 64;
+  if (chunks * pairs >= 2 * sms) {
+    const int items = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, pairs), chunks * pairs / (16 * sms))));
+    KVB_CUDA(launch(kvb::write8_kernel<KIND, D, 64, F16>, dim3(static_cast<unsigned>(chunks * ((pairs + items - 1) / items))),
+                    kvb::W8_THREADS, 0, s, p, items));
+  } else {
+    KVB_CUDA(launch(kvb::write8_kernel<KIND, D, 8, F16>, dim3(static_cast<unsigned>((p.n + 7) / 8 * pairs)), kvb::W8_THREADS, 0, s, p, 1));
+  }
   return KVSKIP_OK;
+}
+
+template <int KIND, int D>
+int by_type(const kvskip_write8_params& p, cudaStream_t s) {
+  return p.x_f16 ? by_chunk<KIND, D, true>(p, s) : by_chunk<KIND, D, false>(p, s);
 }
 
 // CTAs for `n` table or slot entries
@@ -205,11 +214,12 @@ int kvskip_launch_write8(const kvskip_write8_params* p, void* stream) {
     return fail(KVSKIP_E_ARG, "write8: rows of k_new and v_new must be 16-byte aligned");
   if (misaligned(p->k, 8) || misaligned(p->v, 8) || (p->k_sb | p->k_sh | p->k_st | p->v_sb | p->v_sh | p->v_st) % 8)
     return fail(KVSKIP_E_ARG, "write8: rows of k and v must be 8-byte aligned");
-  if (p->Hkv > 65535 || (p->n + 7) / 8 > 2147483647LL) return fail(KVSKIP_E_LIMIT, "write8: grid limits exceeded");
+  if (p->Hkv > 65535 || p->n > 2147483647LL - 64 || (p->n + 63) / 64 * 2 * p->Hkv > 2147483647LL)
+    return fail(KVSKIP_E_LIMIT, "write8: grid limits exceeded (tokens, heads)");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->kind == KVSKIP_KIND_E4M3)
-    return p->D == 128 ? by_chunk<KVSKIP_KIND_E4M3, 128>(*p, s) : by_chunk<KVSKIP_KIND_E4M3, 64>(*p, s);
-  return p->D == 128 ? by_chunk<KVSKIP_KIND_INT8, 128>(*p, s) : by_chunk<KVSKIP_KIND_INT8, 64>(*p, s);
+    return p->D == 128 ? by_type<KVSKIP_KIND_E4M3, 128>(*p, s) : by_type<KVSKIP_KIND_E4M3, 64>(*p, s);
+  return p->D == 128 ? by_type<KVSKIP_KIND_INT8, 128>(*p, s) : by_type<KVSKIP_KIND_INT8, 64>(*p, s);
 }
 
 int kvskip_launch_extend_pages(const kvskip_pages_params* p, void* stream) {
