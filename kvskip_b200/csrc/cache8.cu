@@ -109,19 +109,46 @@ int by_group(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cudaStream
   return launch_decode8<KIND, D, 2>(p, maps, s);
 }
 
+// Map over the new tokens: (D, inner, Hkv, outer), boxes of 16 rows.  False where a stride has no place in one.
+bool token_map(CUtensorMap* map, const kvskip_write8_params& p, const uint16_t* x, int64_t so, int64_t si, int64_t sh) {
+  const auto enc = kvb_host::encode_tiled();
+  const int64_t outer = p.n / p.inner;
+  if (p.inner == 1) si = p.D;
+  if (p.Hkv == 1) sh = p.D;
+  if (outer == 1) so = p.D;
+  if (!enc || si <= 0 || sh <= 0 || so <= 0) return false;
+  const cuuint64_t gdim[4] = {static_cast<cuuint64_t>(p.D), static_cast<cuuint64_t>(p.inner), static_cast<cuuint64_t>(p.Hkv),
+                              static_cast<cuuint64_t>(outer)};
+  const cuuint64_t gstr[3] = {static_cast<cuuint64_t>(si) * 2, static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(so) * 2};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(p.D), 16, 1, 1}, est[4] = {1, 1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t*>(x), gdim, gstr, box, est,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int KIND, int D, bool F16, int CHUNK>
+int launch_write8(const kvskip_write8_params& p, cudaStream_t s) {
+  using Cfg = kvb::W8Cfg<D, CHUNK>;
+  auto kernel = kvb::write8_kernel<KIND, D, CHUNK, F16>;
+  if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmem)) return rc;
+  kvb::W8Maps maps{};
+  const bool tma = token_map(&maps.k, p, p.k_new, p.kn_so, p.kn_si, p.kn_sh) &&
+                   token_map(&maps.v, p, p.v_new, p.vn_so, p.vn_si, p.vn_sh);
+  const int64_t jobs = (p.n + CHUNK - 1) / CHUNK * 2 * p.Hkv;        // one pair each
+  const int64_t ctas = std::min<int64_t>((jobs + Cfg::kWarps - 1) / Cfg::kWarps, kvb_host::num_sms() * (227 * 1024 / Cfg::kSmem));
+  KVB_CUDA(launch(kernel, dim3(static_cast<unsigned>(ctas)), Cfg::kThreads, Cfg::kSmem, s, p, maps, 1, static_cast<int>(jobs),
+                  tma ? 1 : 0));
+  return KVSKIP_OK;
+}
+
 template <int KIND, int D, bool F16>
 int by_chunk(const kvskip_write8_params& p, cudaStream_t s) {
-  // The slots of a CTA: 64 when that still gives every SM work, else 8, so that the tokens of a decode step
-  // spread over the GPU.  Pairs of a CTA: as many as leave 16 CTAs per SM.
-  const int64_t sms = kvb_host::num_sms(), pairs = 2 * static_cast<int64_t>(p.Hkv), chunks = (p.n + 63) / 64;
-  if (chunks * pairs >= 2 * sms) {
-    const int items = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, pairs), chunks * pairs / (16 * sms))));
-    KVB_CUDA(launch(kvb::write8_kernel<KIND, D, 64, F16>, dim3(static_cast<unsigned>(chunks * ((pairs + items - 1) / items))),
-                    kvb::W8_THREADS, 0, s, p, items));
-  } else {
-    KVB_CUDA(launch(kvb::write8_kernel<KIND, D, 8, F16>, dim3(static_cast<unsigned>((p.n + 7) / 8 * pairs)), kvb::W8_THREADS, 0, s, p, 1));
-  }
-  return KVSKIP_OK;
+  // The slots of a warp: 64, or fewer where every warp of the GPU would not get a job, so that the tokens of a decode
+  // step spread over it.  B200, 256 tokens of 8 heads: 4.1 us with 4, 5.8 with 8; prompts of 54k tokens: 59 us with 64.
+  const int64_t warps = static_cast<int64_t>(kvb_host::num_sms()) * kvb::W8Cfg<D, 64>::kWarps, pairs = 2 * p.Hkv;
+  if ((p.n + 63) / 64 * pairs >= warps) return launch_write8<KIND, D, F16, 64>(p, s);
+  if ((p.n + 15) / 16 * pairs >= warps) return launch_write8<KIND, D, F16, 16>(p, s);
+  return launch_write8<KIND, D, F16, 4>(p, s);
 }
 
 template <int KIND, int D>
@@ -139,7 +166,8 @@ int check_pages(const kvskip_pages_params* p, const char* who) {
   if (!p->lens || !p->table || !p->free_pages || !p->n_free || !p->lens_out || !p->n_free_out)
     return fail(KVSKIP_E_ARG, "%s: lens, table, free_pages, n_free, lens_out and n_free_out are required", who);
   if (p->B < 1 || p->max_pages < 1 || p->num_free < 1) return fail(KVSKIP_E_ARG, "%s: B, max_pages, num_free >= 1", who);
-  if (p->max_pages > 2147483647 / KVSKIP_TILE) return fail(KVSKIP_E_LIMIT, "%s: more than 2^31 tokens per request", who);
+  if (p->max_pages > kvb::PG_MOST_PAGES || p->num_free >= 1 << 30)
+    return fail(KVSKIP_E_LIMIT, "%s: at most 2^26 tokens per request, less than 2^30 pages", who);
   return KVSKIP_OK;
 }
 
@@ -204,7 +232,7 @@ int kvskip_launch_write8(const kvskip_write8_params* p, void* stream) {
   if (!p) return fail(KVSKIP_E_ARG, "null parameter block");
   if (p->D != 64 && p->D != 128) return fail(KVSKIP_E_ARG, "write8: head dim 64 or 128");
   if (p->kind != KVSKIP_KIND_E4M3 && p->kind != KVSKIP_KIND_INT8) return fail(KVSKIP_E_ARG, "write8: kind 0 (e4m3) or 1 (int8)");
-  if (p->n < 0 || p->inner < 1 || p->Hkv < 1 || p->blocks < 1 || p->tokens < 1 || p->num_blocks < 1)
+  if (p->n < 0 || p->inner < 1 || p->n % p->inner || p->Hkv < 1 || p->blocks < 1 || p->tokens < 1 || p->num_blocks < 1)
     return fail(KVSKIP_E_ARG, "write8: bad n / inner / Hkv / blocks / tokens / num_blocks");
   if (p->n == 0) return KVSKIP_OK;
   if (!p->k_new || !p->v_new || !p->slots || !p->k || !p->v || !p->k_scale || !p->v_scale)
@@ -214,7 +242,7 @@ int kvskip_launch_write8(const kvskip_write8_params* p, void* stream) {
     return fail(KVSKIP_E_ARG, "write8: rows of k_new and v_new must be 16-byte aligned");
   if (misaligned(p->k, 8) || misaligned(p->v, 8) || (p->k_sb | p->k_sh | p->k_st | p->v_sb | p->v_sh | p->v_st) % 8)
     return fail(KVSKIP_E_ARG, "write8: rows of k and v must be 8-byte aligned");
-  if (p->Hkv > 65535 || p->n > 2147483647LL - 64 || (p->n + 63) / 64 * 2 * p->Hkv > 2147483647LL)
+  if (p->Hkv > 65535 || p->n > 2147483647LL - 64 || (p->n + 3) / 4 * 2 * p->Hkv > 1073741823LL)
     return fail(KVSKIP_E_LIMIT, "write8: grid limits exceeded (tokens, heads)");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->kind == KVSKIP_KIND_E4M3)

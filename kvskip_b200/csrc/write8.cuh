@@ -8,19 +8,17 @@
 // on the arithmetic's last bit.
 //
 // What bounds it: 2 bytes read and 1 written per element: HBM for prompts, the chain slot -> scale so far -> codes for a
-// decode step.  A CTA takes the runs (tokens of one block, consecutive rows) that begin among its CHUNK entries of the
-// slot list, for `items` of the 2 Hkv (head, K or V) pairs.  A few long runs are done by the whole CTA one after the
-// other: the values of a run stay in registers between the maximum and the rounding (one read), and those of the next
-// one are on their way meanwhile.  Many short ones, the tokens of a decode step, are done by a warp each.
+// decode step.  A warp takes the runs (tokens of one block, consecutive rows) that begin among CHUNK entries of the
+// slot list, for `items` of the 2 Hkv (head, K or V) pairs, and needs no other warp: it looks at the slots with ballots,
+// brings a run's values into its own 64 rows of shared memory with TMA, reads them there once for the maximum and
+// once for the codes.  Runs of one token, those of a decode step, are read from global memory directly, two or four an
+// instruction and four or eight at once.
 #pragma once
 #include "common.cuh"
 #include "decode8.cuh"
 
 namespace kvb {
 
-constexpr int W8_THREADS = 256;
-constexpr int W8_WARPS = W8_THREADS / 32;
-constexpr int W8_COOP = 2;             // runs of a chunk up to which the whole CTA works on one run
 constexpr float W8_MIN_SCALE = 7.888609052210118e-31f;   // 2^-100
 
 // Largest magnitude of the 16-bit floats of a 16-byte group and m, two at a time (magnitudes order like their bits).
@@ -74,233 +72,277 @@ __device__ __forceinline__ uint32_t w8_codes(const float a, const float b, const
     return one(a) | (one(b) << 8) | (one(c) << 16) | (one(d) << 24);
   }
 }
-// Eight values x / s, exactly rounded, as codes.  EXACT: by the reciprocal `f` of a power of two, else by s = f itself
-// (a scale that the cache had from elsewhere).
-template <int KIND, bool F16, bool EXACT>
-__device__ __forceinline__ uint2 w8_codes8(const uint4 w, const float f) {
+// Eight values x / s, exactly rounded, as codes: by the reciprocal `inv` of a power of two, or (a scale that the cache had
+// from elsewhere; out of the way of the usual code) by a division.
+template <int KIND, bool F16>
+__device__ __forceinline__ uint2 w8_codes8(const uint4 w, const float inv) {
   const float2 a = w8_pair<F16>(w.x), b = w8_pair<F16>(w.y), c = w8_pair<F16>(w.z), d = w8_pair<F16>(w.w);
-  auto q = [f](const float x) { return EXACT ? x * f : __fdiv_rn(x, f); };
-  return make_uint2(w8_codes<KIND>(q(a.x), q(a.y), q(b.x), q(b.y)), w8_codes<KIND>(q(c.x), q(c.y), q(d.x), q(d.y)));
+  return make_uint2(w8_codes<KIND>(a.x * inv, a.y * inv, b.x * inv, b.y * inv),
+                    w8_codes<KIND>(c.x * inv, c.y * inv, d.x * inv, d.y * inv));
 }
-// four codes times r, rounded again
+template <int KIND, bool F16>
+__device__ __noinline__ uint2 w8_codes8_div(const uint4 w, const float s) {
+  const float2 a = w8_pair<F16>(w.x), b = w8_pair<F16>(w.y), c = w8_pair<F16>(w.z), d = w8_pair<F16>(w.w);
+  return make_uint2(w8_codes<KIND>(__fdiv_rn(a.x, s), __fdiv_rn(a.y, s), __fdiv_rn(b.x, s), __fdiv_rn(b.y, s)),
+                    w8_codes<KIND>(__fdiv_rn(c.x, s), __fdiv_rn(c.y, s), __fdiv_rn(d.x, s), __fdiv_rn(d.y, s)));
+}
+// Rows of a block whose scale has grown, rounded to it: eight codes a lane, rows [row, end) in steps of `rows`.
 template <int KIND>
-__device__ __forceinline__ uint32_t w8_again(const uint32_t w, const float r) {
-  uint32_t x, y;
-  codes_to_f16<KIND, 0>(w, x, y);
-  const float2 a = unpack_f16(x), b = unpack_f16(y);
-  return w8_codes<KIND>(a.x * r, a.y * r, b.x * r, b.y * r);
+__device__ __noinline__ void w8_again(uint8_t* y, const int64_t st, int row, const int end, const int rows, const float ratio) {
+  auto four = [ratio](const uint32_t w) {
+    uint32_t x, z;
+    codes_to_f16<KIND, 0>(w, x, z);
+    const float2 a = unpack_f16(x), b = unpack_f16(z);
+    return w8_codes<KIND>(a.x * ratio, a.y * ratio, b.x * ratio, b.y * ratio);
+  };
+#pragma unroll 4
+  for (; row < end; row += rows) {
+    uint2* at = reinterpret_cast<uint2*>(y + row * st);
+    const uint2 w = *at;
+    *at = make_uint2(four(w.x), four(w.y));
+  }
 }
 
-template <int KIND, int D, int CHUNK, bool F16>
-__global__ void __launch_bounds__(W8_THREADS, 4)
-write8_kernel(const __grid_constant__ kvskip_write8_params p, const int items) {
-  constexpr int LPR = D / 8;                        // lanes of a row, 8 values each
-  constexpr int RPC = W8_THREADS / LPR, RPW = 32 / LPR;   // rows of a pass of the CTA / a warp
-  constexpr int PASSES = TILE / RPC;
-  constexpr int SPAN = CHUNK + TILE;                // slots looked at: the chunk and what a run may reach behind it
-  static_assert(SPAN < W8_THREADS, "one slot a thread");
-  __shared__ int64_t slot[SPAN + 1];                // [0]: the one before the chunk
-  __shared__ uint32_t brk[(SPAN + 31) / 32];        // bit i: slot i does not continue the run of slot i - 1
-  __shared__ int lead[CHUNK], n_lead, longest;
-  __shared__ uint32_t wtop[2][W8_WARPS];
-  __shared__ float wold[2];
+struct W8Maps {
+  CUtensorMap k, v;                      // (D, inner, Hkv, outer) of the new tokens; a box is 16 rows of one head
+};
+template <int D, int CHUNK>
+struct W8Cfg {
+  static constexpr int kWarps = CHUNK == 4 ? 2 : 12;
+  static constexpr int kBatch = CHUNK == 4 ? 4 : 8;          // runs of one token that a warp has in flight
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kStage = TILE * D * 2;                // a run's values
+  static constexpr int kSmem = kWarps * kStage + 128;
+};
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  // Blocks of one chunk follow one another, K heads first: the 2 D bytes that a pair reads of a token lie beside those of
-  // its neighbours, and DRAM pages are opened once for all of them.
-  const int groups = (2 * p.Hkv + items - 1) / items;
-  const int i0 = blockIdx.x / groups * CHUNK, n = static_cast<int>(p.n);
-  const int c0 = blockIdx.x % groups * items, c1 = min(c0 + items, 2 * p.Hkv);     // pairs: K heads, then V heads
-  const bool first = c0 == 0;
+// tma: the tensor maps are valid (all strides positive); jobs: chunks of the slot list times groups of `items` pairs.
+template <int KIND, int D, int CHUNK, bool F16>
+__global__ void __launch_bounds__(W8Cfg<D, CHUNK>::kThreads, 1)
+write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_constant__ W8Maps maps, const int items,
+              const int jobs, const int tma) {
+  using Cfg = W8Cfg<D, CHUNK>;
+  constexpr int NW = Cfg::kWarps;
+  constexpr int LPR = D / 8, RPW = 32 / LPR;        // lanes of a row, 8 values each; rows of an instruction
+  constexpr int WORDS = CHUNK / 32 + (CHUNK % 32 != 0) + 2;   // 32 slots each: the chunk and what a run may reach behind it
   constexpr uint32_t inf = F16 ? 0x7c00u : 0x7f80u;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t bars[NW];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* stage = smem_raw + ((128 - (smem_u32(smem_raw) & 127)) & 127) + warp * Cfg::kStage;
+  uint64_t* bar = &bars[warp];
+  if (lane == 0) mbar_init(bar, 1);
+  mbar_fence_init();
+  __syncwarp();
   pdl_wait_prior();
   pdl_launch_dependents();
 
-  // values of token i (of this chunk's slots), eight channels
-  auto value = [&](const int i, const int c, const int ch) -> uint4 {
-    const uint32_t at = i0 + i, inner = static_cast<uint32_t>(p.inner);
-    const uint32_t o = p.inner == p.n ? 0u : at / inner;
-    const bool v = c >= p.Hkv;
-    const int64_t so = v ? p.vn_so : p.kn_so, si = v ? p.vn_si : p.kn_si, sh = v ? p.vn_sh : p.kn_sh;
-    return __ldg(reinterpret_cast<const uint4*>((v ? p.v_new : p.k_new) + o * so + (at - o * inner) * si + (v ? c - p.Hkv : c) * sh + 8 * ch));
+  const int n = static_cast<int>(p.n), groups = (2 * p.Hkv + items - 1) / items;
+  const uint32_t inner = static_cast<uint32_t>(p.inner);
+  const int ch = lane % LPR, r0 = lane / LPR;
+  uint32_t phase = 0;
+  auto read_slots = [&](const int job, int64_t (&s)[WORDS], int64_t& prev) {
+    const int i0 = job / groups * CHUNK;
+    prev = -1;
+    if (lane == 0 && i0 > 0) prev = p.slots[i0 - 1];
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) {
+      const int at = i0 + k * 32 + lane;
+      s[k] = -1;
+      if (k * 32 + lane < CHUNK + TILE && at < n) s[k] = p.slots[at];
+    }
   };
-  if (tid == 0) n_lead = longest = 0;
-  if (tid <= SPAN) {
-    const int at = i0 + tid - 1;
-    int64_t s = -1;
-    if (at >= 0 && at < n) {
-      s = p.slots[at];
-      // outside the cache: a slot too large, or a row that the contiguous form has no room for
+  const int step = NW * gridDim.x;
+  int job = blockIdx.x * NW + warp;      // (neighbouring warps: the pairs of one chunk, whose values lie side by side)
+  int64_t ahead[WORDS], ahead_prev = -1;
+  if (job < jobs) read_slots(job, ahead, ahead_prev);
+
+  for (; job < jobs; job += step) {
+    const int i0 = job / groups * CHUNK;
+    const int c0 = job % groups * items, c1 = min(c0 + items, 2 * p.Hkv);    // pairs: K heads, then V heads
+    int64_t slot[WORDS], last = ahead_prev;
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) slot[k] = ahead[k];
+    if (job + step < jobs) read_slots(job + step, ahead, ahead_prev);
+
+    // ---- the runs: bit i of brk: slot i does not continue the run of slot i - 1; of lead: a run begins there
+    uint32_t brk[WORDS + 1], lead[WORDS], single[WORDS];
+    auto outside = [&](const int64_t s) {           // a slot too large, or a row the contiguous form has no room for
       bool out = s >= p.num_blocks * TILE;
       if (p.blocks > 1 || p.tokens < TILE) out |= s >= 0 && (s / TILE) % p.blocks * TILE + s % TILE >= p.tokens;
-      if (out) {
-        if (first) atomicCAS(&g_status, 0u, 0x302u);
-        s = -1;
-      }
-    }
-    slot[tid] = s;
-  }
-  __syncthreads();
-  if (tid < ((SPAN + 31) & ~31)) {
-    const bool in = tid < SPAN;
-    const int64_t s = in ? slot[tid + 1] : -1, before = in ? slot[tid] : -1;
-    const bool cont = s >= 0 && before >= 0 && s == before + 1 && (s & (TILE - 1)) != 0;
-    const uint32_t bits = __ballot_sync(0xffffffffu, !cont);
-    if (lane == 0) brk[warp] = bits;
-    if (in && tid < CHUNK && s >= 0 && !cont) {
-      if (before >= 0 && (s >> 6) == (before >> 6)) {      // a second run of the same block
-        if (first) atomicCAS(&g_status, 0u, 0x303u);
-      } else {
-        lead[atomicAdd(&n_lead, 1)] = tid;                 // (the order of the runs does not matter)
-      }
-    }
-  }
-  __syncthreads();
-
-  auto length = [&](const int i) -> int {                  // tokens of the run that begins at i
-    int j = i + 1;
-    while (j < SPAN) {
-      const uint32_t w = brk[j >> 5] >> (j & 31);
-      if (w) return min(j + __ffs(w) - 1, SPAN) - i;
-      j = (j | 31) + 1;
-    }
-    return SPAN - i;                                       // (runs end at the block's last row: at most 64)
-  };
-  struct Run {
-    int i, n, row;
-    int64_t seq, blk;    // sequence (page) and block in it
-  };
-  auto open = [&](const int i) -> Run {
-    Run r;
-    r.i = i;
-    r.n = length(i);
-    const int64_t s = slot[i + 1];
-    r.row = static_cast<int>(s & (TILE - 1));
-    r.seq = s >> 6, r.blk = 0;
-    if (p.blocks > 1) r.blk = r.seq % p.blocks, r.seq /= p.blocks;
-    return r;
-  };
-  auto codes = [&](const Run& r, const int c) -> uint8_t* {
-    return c >= p.Hkv ? p.v + r.seq * p.v_sb + (c - p.Hkv) * p.v_sh + (r.blk * TILE + r.row) * p.v_st
-                      : p.k + r.seq * p.k_sb + c * p.k_sh + (r.blk * TILE + r.row) * p.k_st;
-  };
-  auto scale = [&](const Run& r, const int c) -> float* {
-    return c >= p.Hkv ? p.v_scale + r.seq * p.vs_sb + (c - p.Hkv) * p.vs_sh + r.blk * p.vs_st
-                      : p.k_scale + r.seq * p.ks_sb + c * p.ks_sh + r.blk * p.ks_st;
-  };
-  auto before = [&](const Run& r, const int c) -> float {  // scale of the rows before the run
-    if (r.row == 0) return W8_MIN_SCALE;
-    const float o = *scale(r, c);
-    return o > 0.f && o <= 3.402823466e38f ? o : W8_MIN_SCALE;
-  };
-  // rows before the run, rounded to the larger scale
-  auto again = [&](const Run& r, const int c, const float ratio, const int ch, const int r0, const int step) {
-    const int64_t st = c >= p.Hkv ? p.v_st : p.k_st;
-    for (int row = r0 - r.row; row < 0; row += step) {
-      uint2* y = reinterpret_cast<uint2*>(codes(r, c) + row * st + 8 * ch);
-      const uint2 w = *y;
-      *y = make_uint2(w8_again<KIND>(w.x, ratio), w8_again<KIND>(w.y, ratio));
-    }
-  };
-
-  if (n_lead <= W8_COOP) {
-    if (tid < n_lead) atomicMax(&longest, length(lead[tid]));
-    __syncthreads();
-  }
-  if (n_lead <= W8_COOP && longest > 2 * RPW) {
-    const int ch = tid % LPR, r0 = tid / LPR;
-    const Run run0 = open(lead[0]), run1 = open(lead[n_lead - 1]);
-    const int jobs = (c1 - c0) * n_lead;
-    // (a run that goes on in the next row of a padded list has no one stride)
-    const uint32_t inner = static_cast<uint32_t>(p.inner);
-    auto fetch = [&](const int j, uint4 (&x)[PASSES], float& old) {
-      const Run& r = j % n_lead ? run1 : run0;
-      const int c = c0 + j / n_lead;
-      const uint32_t at = i0 + r.i, o = inner == static_cast<uint32_t>(n) ? 0u : at / inner, in = at - o * inner;
-      if (in + r.n <= inner) {
-        const bool v = c >= p.Hkv;
-        const int64_t si = v ? p.vn_si : p.kn_si;
-        const uint16_t* src = v ? p.v_new + o * p.vn_so + (c - p.Hkv) * p.vn_sh : p.k_new + o * p.kn_so + c * p.kn_sh;
-        src += (in + r0) * si + 8 * ch;
-#pragma unroll
-        for (int q = 0; q < PASSES; ++q) {
-          x[q] = make_uint4(0u, 0u, 0u, 0u);
-          if (q * RPC + r0 < r.n) x[q] = __ldg(reinterpret_cast<const uint4*>(src + q * RPC * si));
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < PASSES; ++q) {
-          x[q] = make_uint4(0u, 0u, 0u, 0u);
-          if (q * RPC + r0 < r.n) x[q] = value(r.i + q * RPC + r0, c, ch);
-        }
-      }
-      if (tid == 0) old = before(r, c);
+      return out;
     };
-    auto work = [&](const int j, const uint4 (&x)[PASSES], const float old) {
-      const Run& r = j % n_lead ? run1 : run0;
-      const int c = c0 + j / n_lead;
-      uint32_t top = 0;
+    if (outside(last)) last = -1;
 #pragma unroll
-      for (int q = 0; q < PASSES; ++q) top = w8_top(top, x[q]);
-      if (max(top & 0xffffu, top >> 16) >= inf) {
-        top = 0;
-#pragma unroll
-        for (int q = 0; q < PASSES; ++q) top = w8_top_finite(top, x[q], inf);
+    for (int k = 0; k < WORDS; ++k) {
+      const bool in = k * 32 + lane < CHUNK;
+      if (outside(slot[k])) {
+        if (in && c0 == 0) atomicCAS(&g_status, 0u, 0x302u);
+        slot[k] = -1;
       }
-      top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-      if (lane == 0) wtop[j & 1][warp] = top;
-      if (tid == 0) wold[j & 1] = old;
-      __syncthreads();
+      int64_t before = __shfl_up_sync(0xffffffffu, slot[k], 1);
+      if (lane == 0) before = last;
+      last = __shfl_sync(0xffffffffu, slot[k], 31);
+      const bool some = slot[k] >= 0;
+      const bool cont = some && before >= 0 && slot[k] == before + 1 && (slot[k] & (TILE - 1)) != 0;
+      const bool twice = some && !cont && before >= 0 && (slot[k] >> 6) == (before >> 6);   // a second run of the block
+      if (twice && in && c0 == 0) atomicCAS(&g_status, 0u, 0x303u);
+      brk[k] = __ballot_sync(0xffffffffu, !cont);
+      lead[k] = __ballot_sync(0xffffffffu, some && !cont && !twice && in);
+    }
+    brk[WORDS] = 0xffffffffu;
 #pragma unroll
-      for (int w = 0; w < W8_WARPS; ++w) top = max(top, wtop[j & 1][w]);
-      const float was = wold[j & 1], s = fmaxf(was, w8_scale<KIND, F16>(top));
-      const float inv = w8_inverse(s);
-      const int64_t st = c >= p.Hkv ? p.v_st : p.k_st;
-      uint8_t* y = codes(r, c) + r0 * st + 8 * ch;
-      if (inv != 0.f) {
-#pragma unroll
-        for (int q = 0; q < PASSES; ++q)
-          if (q * RPC + r0 < r.n) *reinterpret_cast<uint2*>(y + q * RPC * st) = w8_codes8<KIND, F16, true>(x[q], inv);
-      } else {
-#pragma unroll
-        for (int q = 0; q < PASSES; ++q)
-          if (q * RPC + r0 < r.n) *reinterpret_cast<uint2*>(y + q * RPC * st) = w8_codes8<KIND, F16, false>(x[q], s);
-      }
-      if (r.row > 0 && s > was) again(r, c, __fdiv_rn(was, s), ch, r0, RPC);
-      if (tid == 0) *scale(r, c) = s;
+    for (int k = 0; k < WORDS; ++k) single[k] = lead[k] & __funnelshift_r(brk[k], brk[k + 1], 1);   // the next slot breaks too
+    struct Run {
+      int i, n, row;
+      int64_t seq, blk;    // sequence (page) and block in it
     };
-    uint4 x[PASSES], y[PASSES];
-    float ox = 0.f, oy = 0.f;
-    fetch(0, x, ox);
-    for (int j = 0; j < jobs; j += 2) {
-      if (j + 1 < jobs) fetch(j + 1, y, oy);
-      work(j, x, ox);
-      if (j + 1 == jobs) break;
-      if (j + 2 < jobs) fetch(j + 2, x, ox);
-      work(j + 1, y, oy);
-    }
-    return;
-  }
-  for (int k = warp; k < n_lead; k += W8_WARPS) {
-    const Run r = open(lead[k]);
-    const int ch = lane % LPR, r0 = lane / LPR;
-    for (int c = c0; c < c1; ++c) {
-      const float was = before(r, c);
-      uint32_t top = 0;
-      for (int q = r0; q < r.n; q += RPW) top = w8_top_finite(top, value(r.i + q, c, ch), inf);
-      top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-      const float s = fmaxf(was, w8_scale<KIND, F16>(top));
-      const float inv = w8_inverse(s);
-      uint8_t* y = codes(r, c) + 8 * ch;
-      const int64_t st = c >= p.Hkv ? p.v_st : p.k_st;
-      for (int q = r0; q < r.n; q += RPW) {
-        const uint4 x = value(r.i + q, c, ch);
-        *reinterpret_cast<uint2*>(y + q * st) = inv != 0.f ? w8_codes8<KIND, F16, true>(x, inv) : w8_codes8<KIND, F16, false>(x, s);
+    auto open = [&](const int k, const int bit) -> Run {
+      Run r;
+      r.i = k * 32 + bit;
+      r.n = 0;
+      int64_t s = 0;
+#pragma unroll
+      for (int x = 0; x < WORDS; ++x) {
+        const int64_t v = __shfl_sync(0xffffffffu, slot[x], bit);
+        if (x == k) s = v;
+        // tokens up to the next break (a run ends with its block, at most 64 tokens on)
+        const uint32_t w = x < k ? 0u : x == k ? brk[x] & ~((2u << bit) - 1u) : brk[x];
+        if (r.n == 0 && w) r.n = x * 32 + __ffs(w) - 1 - r.i;
       }
-      if (r.row > 0 && s > was) again(r, c, __fdiv_rn(was, s), ch, r0, RPW);
-      __syncwarp();                        // (every lane has read the old scale)
-      if (lane == 0) *scale(r, c) = s;
-    }
+      if (r.n == 0) r.n = WORDS * 32 - r.i;
+      r.row = static_cast<int>(s & (TILE - 1));
+      r.seq = s >> 6, r.blk = 0;
+      if (p.blocks > 1) r.blk = r.seq % p.blocks, r.seq /= p.blocks;
+      return r;
+    };
+    auto source = [&](const uint32_t at, const int c) -> const uint16_t* {    // values of one token
+      const uint32_t o = inner == static_cast<uint32_t>(n) ? 0u : at / inner, in = at - o * inner;
+      return c >= p.Hkv ? p.v_new + o * p.vn_so + in * p.vn_si + (c - p.Hkv) * p.vn_sh : p.k_new + o * p.kn_so + in * p.kn_si + c * p.kn_sh;
+    };
+    auto codes = [&](const Run& r, const int c) -> uint8_t* {
+      return c >= p.Hkv ? p.v + r.seq * p.v_sb + (c - p.Hkv) * p.v_sh + (r.blk * TILE + r.row) * p.v_st
+                        : p.k + r.seq * p.k_sb + c * p.k_sh + (r.blk * TILE + r.row) * p.k_st;
+    };
+    auto scale = [&](const Run& r, const int c) -> float* {
+      return c >= p.Hkv ? p.v_scale + r.seq * p.vs_sb + (c - p.Hkv) * p.vs_sh + r.blk * p.vs_st
+                        : p.k_scale + r.seq * p.ks_sb + c * p.ks_sh + r.blk * p.ks_st;
+    };
+    auto usable = [](const float o) { return o > 0.f && o <= 3.402823466e38f ? o : W8_MIN_SCALE; };
+    // rows before the run, rounded to the larger scale
+    auto again = [&](const Run& r, const int c, const float ratio, const int row0, const int rows) {
+      const int64_t st = c >= p.Hkv ? p.v_st : p.k_st;
+      w8_again<KIND>(codes(r, c) - r.row * st + 8 * ch, st, row0, r.row, rows, ratio);
+    };
+    auto put = [&](uint8_t* y, const uint4 x, const float s, const float inv) {
+      *reinterpret_cast<uint2*>(y) = inv != 0.f ? w8_codes8<KIND, F16>(x, inv) : w8_codes8_div<KIND, F16>(x, s);
+    };
+
+    // ---- runs of several tokens
+#pragma unroll
+    for (int k = 0; k < (CHUNK + 31) / 32; ++k)
+      for (uint32_t rest = lead[k] & ~single[k]; rest; rest &= rest - 1) {
+        const Run r = open(k, __ffs(rest) - 1);
+        const uint32_t at = i0 + r.i, o = inner == static_cast<uint32_t>(n) ? 0u : at / inner, in = at - o * inner;
+        const bool staged = tma && in + r.n <= inner;      // (a run may go on in the next row of a padded list)
+        for (int c = c0; c < c1; ++c) {
+          const bool v = c >= p.Hkv;
+          float was = W8_MIN_SCALE;
+          if (r.row > 0) was = *scale(r, c);
+          if (staged && lane == 0) {
+            const int boxes = (r.n + 15) / 16;
+            mbar_expect_tx(bar, boxes * 16 * D * 2);
+            for (int x = 0; x < boxes; ++x)
+              tma_load_4d(stage + x * 16 * D * 2, v ? &maps.v : &maps.k, bar, 0, in + 16 * x, v ? c - p.Hkv : c, o);
+          }
+          was = usable(was);
+          uint32_t top = 0;
+          const uint4* mine = reinterpret_cast<const uint4*>(stage) + lane;     // row r0, then every RPW-th
+          if (staged) {
+            if (!mbar_wait(bar, phase, 0x640u + warp)) return;
+            phase ^= 1;
+            const int full = r.n / RPW;
+            int q = 0;
+            for (; q + 8 <= full; q += 8)
+#pragma unroll
+              for (int u = 0; u < 8; ++u) top = w8_top(top, mine[(q + u) * 32]);
+            for (; q * RPW + r0 < r.n; ++q) top = w8_top(top, mine[q * 32]);
+            if (__any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) >= inf)) {
+              top = 0;
+              for (q = 0; q * RPW + r0 < r.n; ++q) top = w8_top_finite(top, mine[q * 32], inf);
+            }
+          } else {
+            for (int q = r0; q < r.n; q += RPW)
+              top = w8_top_finite(top, *reinterpret_cast<const uint4*>(source(at + q, c) + 8 * ch), inf);
+          }
+          top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+          const float s = fmaxf(was, w8_scale<KIND, F16>(top)), inv = w8_inverse(s);
+          const int64_t st = v ? p.v_st : p.k_st;
+          uint8_t* y = codes(r, c) + r0 * st + 8 * ch;
+          if (staged && inv != 0.f) {
+            const int full = r.n / RPW;
+            int q = 0;
+            for (; q + 4 <= full; q += 4, y += 4 * RPW * st)
+#pragma unroll
+              for (int u = 0; u < 4; ++u) *reinterpret_cast<uint2*>(y + u * RPW * st) = w8_codes8<KIND, F16>(mine[(q + u) * 32], inv);
+            for (; q * RPW + r0 < r.n; ++q, y += RPW * st) *reinterpret_cast<uint2*>(y) = w8_codes8<KIND, F16>(mine[q * 32], inv);
+          } else {
+            for (int q = r0; q < r.n; q += RPW, y += RPW * st)
+              put(y, staged ? mine[(q - r0) / RPW * 32] : *reinterpret_cast<const uint4*>(source(at + q, c) + 8 * ch), s, inv);
+          }
+          if (r.row > 0 && s > was) again(r, c, __fdiv_rn(was, s), r0, RPW);
+          __syncwarp();                    // the stage has been read, and the old scale by every lane
+          if (lane == 0) *scale(r, c) = s;
+        }
+      }
+
+    // ---- runs of one token: lanes r0 = 0 .. RPW - 1 take one each, kBatch / RPW of them at once
+    constexpr int U = Cfg::kBatch / RPW;
+    for (int c = c0; c < c1; ++c)
+#pragma unroll
+      for (int k = 0; k < (CHUNK + 31) / 32; ++k)
+        for (uint32_t rest = single[k]; rest;) {
+          Run r[U];
+          uint4 x[U];
+          float was[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            r[u].i = -1;
+#pragma unroll
+            for (int m = 0; m < RPW; ++m) {
+              const int bit = rest ? __ffs(rest) - 1 : 0;
+              const int64_t s = __shfl_sync(0xffffffffu, slot[k], bit);
+              if (m == r0 && rest) {
+                r[u].i = k * 32 + bit, r[u].n = 1;
+                r[u].row = static_cast<int>(s & (TILE - 1));
+                r[u].seq = s >> 6, r[u].blk = 0;
+                if (p.blocks > 1) r[u].blk = r[u].seq % p.blocks, r[u].seq /= p.blocks;
+              }
+              rest &= rest - 1;
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            x[u] = make_uint4(0u, 0u, 0u, 0u);
+            was[u] = W8_MIN_SCALE;
+            if (r[u].i >= 0) {
+              x[u] = *reinterpret_cast<const uint4*>(source(i0 + r[u].i, c) + 8 * ch);
+              if (r[u].row > 0) was[u] = *scale(r[u], c);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            uint32_t top = w8_top_finite(0u, x[u], inf);
+            top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+            for (int d = LPR / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (r[u].i >= 0) {
+              const float old = usable(was[u]), s = fmaxf(old, w8_scale<KIND, F16>(top));
+              put(codes(r[u], c) + 8 * ch, x[u], s, w8_inverse(s));
+              if (r[u].row > 0 && s > old) again(r[u], c, __fdiv_rn(old, s), 0, 1);
+              if (ch == 0) *scale(r[u], c) = s;
+            }
+          }
+        }
   }
 }
 

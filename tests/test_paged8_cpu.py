@@ -92,7 +92,8 @@ def test_write8_entry_refuses(lib, change, text):
     ("extend_pages", dict(lens=0), b"required"), ("extend_pages", dict(new_=0), b"required"),
     ("extend_pages", dict(slots=0), b"required"), ("extend_pages", dict(B=0), b">= 1"),
     ("extend_pages", dict(per_row=3), b"per_row"), ("extend_pages", dict(n_tokens=-1), b"n_tokens"),
-    ("extend_pages", dict(max_pages=1 << 27), b"2^31"), ("release_pages", dict(done=0), b"done"),
+    ("extend_pages", dict(max_pages=(1 << 20) + 1), b"2^26"),
+    ("release_pages", dict(num_free=1 << 30), b"2^30"), ("release_pages", dict(done=0), b"done"),
     ("release_pages", dict(free_pages=0), b"required")])
 def test_pages_entries_refuse(lib, fn, change, text):
     p = cabi.PagesParams()
