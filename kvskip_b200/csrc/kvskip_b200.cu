@@ -432,8 +432,14 @@ int fail(int code, const char* fmt, ...) {
 int ensure_smem(const void* func, int bytes) { return ::ensure_smem(func, bytes); }
 bool use_pdl() { return g_use_pdl.load(std::memory_order_relaxed) != 0; }
 int num_sms() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static std::atomic<int> known[kMaxDevices];      // 0: not asked for yet (the query costs host time on every call)
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  int sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms < 1) return 148;
+    known[dev].store(sms, std::memory_order_relaxed);
+  }
   return sms;
 }
 EncodeTiledFn encode_tiled() { return encode_tiled_fn(); }

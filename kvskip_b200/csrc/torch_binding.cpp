@@ -8,12 +8,16 @@
 // checks, kvskip_ext.cpp:12-19,29-42,212-221,276-313), allocates outputs and scratch with the
 // caching allocator, and launches on the current stream of the inputs' device.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
 #include <cmath>
+#include <cstdlib>
+#include <cstring>
 #include <limits>
 
 #include "../../include/kvskip_b200.h"
@@ -743,6 +747,15 @@ int check_cache8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
   same_device(k, {&v, &ks, &vs});
   return kind;
 }
+// at::empty without the dispatcher's share of host time: a small call of this section is as long as its host side
+at::Tensor new_cuda(at::IntArrayRef shape, at::ScalarType type, const at::Device& device) {
+  return at::detail::empty_cuda(shape, type, device, c10::nullopt);
+}
+// whether every front-end call is to check the status word (the variable may change while the process runs)
+bool check_wanted() {
+  const char* e = std::getenv("KVSKIP_CHECK_STATUS");
+  return e && *e && std::strcmp(e, "0") != 0;
+}
 uint8_t* u8(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
 // [out of q's type [B,Hq,D], lse [B,Hq], blk_max, blk_sum ([B,Hq,nb] or undefined), out_f32 or undefined]
@@ -795,12 +808,12 @@ std::vector<at::Tensor> decode8(const at::Tensor& q, const at::Tensor& k, const 
     p.max_blocks = static_cast<int32_t>(block_idx->size(2));
     same_device(q, {&*block_idx, &*block_cnt});
   }
-  const auto f32 = q.options().dtype(at::kFloat);
-  at::Tensor out = at::empty({B, Hq, D}, q.options()), lse = at::empty({B, Hq}, f32), out32, bmax, bsum;
-  if (want_f32) out32 = at::empty({B, Hq, D}, f32);
+  const at::Device device = q.device();
+  at::Tensor out = new_cuda({B, Hq, D}, q.scalar_type(), device), lse = new_cuda({B, Hq}, at::kFloat, device), out32, bmax, bsum;
+  if (want_f32) out32 = new_cuda({B, Hq, D}, at::kFloat, device);
   if (stats) {
-    bmax = at::empty({B, Hq, nb}, f32);
-    bsum = at::empty({B, Hq, nb}, f32);
+    bmax = new_cuda({B, Hq, nb}, at::kFloat, device);
+    bsum = new_cuda({B, Hq, nb}, at::kFloat, device);
     p.blk_max = bmax.data_ptr<float>();
     p.blk_sum = bsum.data_ptr<float>();
   }
@@ -822,8 +835,8 @@ std::vector<at::Tensor> decode8(const at::Tensor& q, const at::Tensor& k, const 
   p.out = u16m(out);
   if (want_f32) p.out_f32 = out32.data_ptr<float>();
   p.lse = lse.data_ptr<float>();
-  const at::Tensor work = at::empty({kvskip_decode8_work_bytes(&p)}, q.options().dtype(at::kByte));
-  p.work = work.data_ptr();
+  const c10::DataPtr work = c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(kvskip_decode8_work_bytes(&p)));
+  p.work = work.get();
   raise_on(kvskip_launch_decode8(&p, cur_stream()));
   return {out, lse, bmax, bsum, out32};
 }
@@ -887,8 +900,8 @@ void fill_pages(kvskip_pages_params& p, const at::Tensor& lens, const at::Tensor
                   page_table.size(1) >= 1, "lens: [B], page_table: [B, max_pages]");
   TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) >= 1 && n_free.numel() == 1, "free_pages: [pages], n_free: one element");
   same_device(lens, {&page_table, &free_pages, &n_free});
-  lo = lens_out.has_value() ? *lens_out : at::empty_like(lens);
-  fo = n_free_out.has_value() ? *n_free_out : at::empty_like(n_free);
+  lo = lens_out.has_value() ? *lens_out : new_cuda(lens.sizes(), at::kInt, lens.device());
+  fo = n_free_out.has_value() ? *n_free_out : new_cuda(n_free.sizes(), at::kInt, lens.device());
   p.lens_out = const_cast<int32_t*>(i32(lo, "lens_out"));
   p.n_free_out = const_cast<int32_t*>(i32(fo, "n_free_out"));
   TORCH_CHECK(lo.numel() == lens.numel() && fo.numel() == 1, "lens_out: [B], n_free_out: one element");
@@ -917,10 +930,11 @@ std::vector<at::Tensor> extend_pages(const at::Tensor& lens, const at::Tensor& n
   TORCH_CHECK(per_row >= 0 && n_tokens >= 0 && (per_row == 0 || per_row <= std::numeric_limits<int32_t>::max()),
               "extend_pages: n_tokens or per_row");
   const int64_t n = per_row ? B * per_row : n_tokens;
-  const std::vector<int64_t> shape = per_row ? std::vector<int64_t>{B, per_row} : std::vector<int64_t>{n};
-  at::Tensor slots = at::empty(shape, lens.options().dtype(at::kLong));
-  at::Tensor positions = at::empty(shape, lens.options());
-  at::Tensor granted = at::empty({B}, lens.options().dtype(at::kBool));
+  const int64_t dims[2] = {per_row ? B : n, per_row};
+  const at::IntArrayRef shape(dims, per_row ? 2 : 1);
+  at::Tensor slots = new_cuda(shape, at::kLong, lens.device());
+  at::Tensor positions = new_cuda(shape, at::kInt, lens.device());
+  at::Tensor granted = new_cuda({B}, at::kBool, lens.device());
   p.slots = slots.data_ptr<int64_t>();
   p.positions = positions.data_ptr<int32_t>();
   p.granted = static_cast<uint8_t*>(granted.data_ptr());
@@ -1025,6 +1039,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("t_dev") = py::none(), py::arg("T_bound") = 0);
   m.def("advance", &advance, "device-resident sequence length += delta, in stream order", py::arg("t_dev"),
         py::arg("delta") = 1);
+  m.def("check_wanted", &check_wanted, "whether KVSKIP_CHECK_STATUS asks for a check of the status word after every call");
   m.def("decode8", &decode8, "attention of one token per sequence over a cache of 8-bit codes with block scales",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("k_scale"), py::arg("v_scale"), py::arg("scale"),
         py::arg("lens") = py::none(), py::arg("page_table") = py::none(), py::arg("max_len") = 0,

@@ -352,10 +352,12 @@ def decode8(q, k, v, k_scale, v_scale, scale: float, *, lens: torch.Tensor | Non
     Returns dict(out of q's type, lse fp32 [B,Hq][, blk_max, blk_sum fp32 [B,Hq,nb]][, out_f32])."""
     if q.dim() == 4:
         q = q.squeeze(2)
+    e = _EXT or ext()
     bi, bc = (None, None) if plan is None else (plan.block_idx, plan.block_cnt)
-    out, lse, bmax, bsum, o32 = ext().decode8(q, k, v, k_scale, v_scale, scale, lens, page_table, max_len or 0, bi, bc,
-                                              stats, out_f32)
-    _auto_check("decode8")
+    out, lse, bmax, bsum, o32 = e.decode8(q, k, v, k_scale, v_scale, scale, lens, page_table, max_len or 0, bi, bc, stats,
+                                          out_f32)
+    if e.check_wanted():
+        check_status("decode8")
     res = {"out": out, "lse": lse}
     if stats:
         res["blk_max"], res["blk_sum"] = bmax, bsum
@@ -374,8 +376,10 @@ def write8(k_new, v_new, slots, k, v, k_scale, v_scale) -> None:
     makes it grow, the codes already there are rounded to the new scale.  A token in row 0 starts its block
     afresh, whatever page and scale held before.  Infinities saturate; a NaN stays one in e4m3 and is 0 in int8.
     A slot outside the cache is skipped and sets the status word (`check_status`)."""
-    ext().write8(k_new, v_new, slots, k, v, k_scale, v_scale)
-    _auto_check("write8")
+    e = _EXT or ext()
+    e.write8(k_new, v_new, slots, k, v, k_scale, v_scale)
+    if e.check_wanted():
+        check_status("write8")
 
 
 def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | None = None, per_row: int | None = None,
@@ -394,7 +398,7 @@ def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | N
         raise ValueError("extend_pages: either n_tokens (packed) or per_row (padded)")
     if per_row is not None and per_row < 1:
         raise ValueError("extend_pages: per_row >= 1")
-    slots, positions, granted, lens2, n2 = ext().extend_pages(lens, new, page_table, free_pages, n_free, n_tokens or 0,
+    slots, positions, granted, lens2, n2 = (_EXT or ext()).extend_pages(lens, new, page_table, free_pages, n_free, n_tokens or 0,
                                                               per_row or 0, lens_out, n_free_out)
     return {"slots": slots, "positions": positions, "granted": granted, "lens": lens2, "n_free": n2}
 
@@ -404,5 +408,5 @@ def release_pages(done, lens, page_table, free_pages, n_free, *, lens_out: torch
     """The pages of the requests marked in `done` (bool or uint8 [B]) go back to the stack of
     `extend_pages` and their lengths become 0 (the table is left as it is).  Returns dict(lens, n_free), new
     tensors unless lens_out / n_free_out are given."""
-    lens2, n2 = ext().release_pages(done, lens, page_table, free_pages, n_free, lens_out, n_free_out)
+    lens2, n2 = (_EXT or ext()).release_pages(done, lens, page_table, free_pages, n_free, lens_out, n_free_out)
     return {"lens": lens2, "n_free": n2}
