@@ -215,9 +215,9 @@ int kvskip_launch_decode8(const kvskip_decode8_params* p, void* stream) {
     return fail(KVSKIP_E_ARG, "decode8: misaligned out / out_f32 / work");
   if (misaligned(p->k, 16) || misaligned(p->v, 16) || (p->k_sb | p->k_sh | p->k_st | p->v_sb | p->v_sh | p->v_st) % 16)
     return fail(KVSKIP_E_ARG, "decode8: k / v must be 16-byte aligned, with strides that are multiples of 16");
-  if (static_cast<int64_t>(p->B) * p->Hkv * (p->block_idx ? std::max(p->max_blocks, p->nb) : p->nb) > 2147483647LL ||
+  if (static_cast<int64_t>(p->B) * p->Hkv * (p->block_idx ? std::max(p->max_blocks, p->nb) : p->nb) > 1 << 29 ||
       static_cast<int64_t>(p->B) * p->Hq > 2147483647LL)
-    return fail(KVSKIP_E_LIMIT, "decode8: more than 2^31 blocks of heads in a call");
+    return fail(KVSKIP_E_LIMIT, "decode8: more than 2^29 blocks of heads in a call");
   kvb::D8Maps maps;
   const int n = p->page_table ? p->num_pages : p->B, rows = p->page_table ? KVSKIP_TILE : p->T;
   if (int rc = make_map(&maps.k, p->k, p->k_sb, p->k_sh, p->k_st, n, p->Hkv, rows, p->D)) return rc;

@@ -49,15 +49,22 @@ struct D8Cfg {
 
 constexpr float D8_PSCALE = 13.f;   // log2 of the scaling of P
 
-// The chunks of the work list.  Every warp has one chunk to begin with.  Under a saturated memory SMs differ by up to a
-// third in the bandwidth they get (by their place on the die), so with enough items per warp the first chunks are five
-// eighths of the list only; two eighths are cut into one more chunk per warp and the last eighth into two, which
-// the warps take from a counter as they get there.
-constexpr int D8_SHARE_MIN = 24;     // items per warp from which on chunks are taken from the counter
-struct D8Zone {                      // items from `base` on, cut into the chunks from `first` on: the first `longer` of
-  uint32_t base, first, size, longer;   // them hold size + 1, the others size
-  __device__ __forceinline__ D8Zone(uint32_t base_, uint32_t items, uint32_t first_, uint32_t chunks)
-      : base(base_), first(first_), size(chunks ? items / chunks : 0), longer(items - size * chunks) {}
+// The chunks of the work list.  Places in the list are costs: a block counts 4, and where heads are short (64 blocks on
+// average) and a warp has at least four blocks, the first block of a head D8_HEAD more (q is read and converted there, and
+// the output written at the end: 2.7 us per block of a long head, 3.7 us per head of one block, measured with every warp
+// of a B200 at work; a ragged batch of 64 takes 45 us with it, 50 without).  A block belongs to the chunk in which it
+// begins.  Every warp has one chunk to begin with.  Under a saturated memory SMs differ in the bandwidth
+// they get (by their place on the die), so with enough blocks per warp the first chunks are five eighths of the list
+// only; two eighths are cut into one more chunk per warp and the last eighth into two, which the warps take from a
+// counter as they get there (batch 16 / 64k: 335 -> 318 us; with 11 blocks per warp it costs more than it gives).
+constexpr int D8_COST = 4, D8_HEAD = 2;
+constexpr int D8_HEAD_MIN = 4;       // blocks per warp from which on heads are counted,
+constexpr int D8_HEAD_MAX = 64;      // and the mean length of a head up to which they are
+constexpr int D8_SHARE_MIN = 24;     // blocks per warp from which on chunks are taken from the counter
+struct D8Zone {                      // costs from `base` on, cut into the chunks from `first` on: the first `longer` of
+  uint32_t base, first, size, longer;   // them have size + 1, the others size
+  __device__ __forceinline__ D8Zone(uint32_t base_, uint32_t costs, uint32_t first_, uint32_t chunks)
+      : base(base_), first(first_), size(chunks ? costs / chunks : 0), longer(costs - size * chunks) {}
   __device__ __forceinline__ uint32_t edge(const uint32_t i) const { return base + size * (i - first) + min(i - first, longer); }
   __device__ __forceinline__ uint32_t of(uint32_t x) const {
     x -= base;
@@ -65,27 +72,29 @@ struct D8Zone {                      // items from `base` on, cut into the chunk
     return first + (x < split ? x / (size + 1) : longer + (x - split) / size);
   }
 };
+// W blocks in `heads` heads.  Every chunk is at least as long as the longest block, so none is empty.
 struct D8Chunks {
-  uint32_t wb, wc, na, nb, nc;       // items and chunks of the shared zones
+  uint32_t head, all;                // cost of a head's beginning, of everything
+  uint32_t wb, wc, na, nb, nc;       // costs and chunks of the shared zones
   D8Zone a, b, c;
-  __device__ __forceinline__ D8Chunks(const uint32_t W, const uint32_t warps, const int, const bool share)
-      : wb(share ? W / 4 : 0), wc(share ? W / 8 : 0), na(min(W, warps)), nb(min(wb / 3, warps)), nc(min(wc / 3, 2 * warps)),
-        a(0, W - wb - wc, 0, na), b(W - wb - wc, wb, na, nb), c(W - wc, wc, na + nb, nc) {}
-  __device__ __forceinline__ D8Chunks(const uint32_t W, const uint32_t warps, const bool counter)
-      : D8Chunks(W, warps, 0, counter && W / D8_SHARE_MIN >= warps) {}
+  __device__ __forceinline__ D8Chunks(const uint32_t W, const uint32_t heads, const uint32_t warps, const bool counter)
+      : head(W / D8_HEAD_MIN >= warps && W / D8_HEAD_MAX < heads ? D8_HEAD : 0), all(W * D8_COST + heads * head),
+        wb(counter && W / D8_SHARE_MIN >= warps ? all / 4 : 0), wc(wb / 2), na(min(W, warps)),
+        nb(min(wb / (3 * D8_COST), warps)), nc(min(wc / (3 * D8_COST), 2 * warps)),
+        a(0, all - wb - wc, 0, na), b(all - wb - wc, wb, na, nb), c(all - wc, wc, na + nb, nc) {}
   __device__ __forceinline__ uint32_t count() const { return na + nb + nc; }
-  // items [begin, end) of chunk i
-  __device__ __forceinline__ void range(const uint32_t i, int& begin, int& end) const {
-    const D8Zone z = i < b.first ? a : i < c.first ? b : c;
-    begin = static_cast<int>(z.edge(i)), end = static_cast<int>(z.edge(i + 1));
+  __device__ __forceinline__ uint32_t edge(const uint32_t i) const {       // where chunk i begins; i <= count()
+    return i < b.first ? a.edge(i) : i < c.first ? b.edge(i) : nc ? c.edge(i) : all;
   }
-  __device__ __forceinline__ uint32_t of(const uint32_t x) const {
-    const D8Zone z = x < b.base ? a : x < c.base ? b : c;
-    return z.of(x);
+  __device__ __forceinline__ uint32_t of(const uint32_t x) const { return x < b.base ? a.of(x) : x < c.base ? b.of(x) : c.of(x); }
+  // first cost of block j of a head, and the first block that begins at or behind cost r of one
+  __device__ __forceinline__ uint32_t at(const uint32_t j) const { return j ? head + j * D8_COST : 0; }
+  __device__ __forceinline__ uint32_t block(const uint32_t r) const {
+    return r == 0 ? 0 : r <= head + D8_COST ? 1 : (r - head + D8_COST - 1) / D8_COST;
   }
 };
-// Layout of `work`: [0] the counter, [4..] items before every unit of the list, then the pieces (two per chunk).
-__host__ __device__ inline int64_t d8_piece_base(const int64_t units) { return (4 + units + 1 + 3) / 4 * 4; }
+// Layout of `work`: [0] the counter, [4..] blocks and heads before every unit of the list, then the pieces (two per chunk).
+__host__ __device__ inline int64_t d8_piece_base(const int64_t units) { return (4 + 2 * (units + 1) + 3) / 4 * 4; }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -142,20 +151,57 @@ __device__ __forceinline__ int d8_count(const kvskip_decode8_params& p, int u) {
   return (d8_len(p, u) + TILE - 1) / TILE;
 }
 
-// Item x of the list; pref[t]: items before the units of thread t's share (pref[THREADS]: all of them).
+// pref[t]: blocks (x) and heads (y) before the units of thread t's share; pref[THREADS]: all of them.
+// The last t with x * cx + y * cy <= key; the whole warp asks for the same key.
 template <int THREADS>
-__device__ __forceinline__ D8Item d8_item(const kvskip_decode8_params& p, const int* pref, const int per, const int x) {
+__device__ __forceinline__ int d8_find(const int2* pref, const uint32_t key, const uint32_t cx, const uint32_t cy) {
+  constexpr int N = THREADS / 32;
+  static_assert(THREADS % 32 == 0 && N <= 32, "two rounds");
+  const int lane = threadIdx.x & 31;
+  auto below = [&](const int t) { return static_cast<uint32_t>(pref[t].x) * cx + static_cast<uint32_t>(pref[t].y) * cy <= key; };
+  const int base = (31 - __clz(__ballot_sync(0xffffffffu, below(lane * N)))) * N;
+  return base + 31 - __clz(__ballot_sync(0xffffffffu, lane < N && below(base + lane)));
+}
+// Number of the first block that begins at or behind cost e.
+template <int THREADS>
+__device__ __forceinline__ int d8_first(const kvskip_decode8_params& p, const D8Chunks& cut, const int2* pref, const int per,
+                                        const uint32_t e) {
+  if (cut.head == 0) return static_cast<int>((e + D8_COST - 1) / D8_COST);
+  if (e >= cut.all) return pref[THREADS].x;
+  const int lo = d8_find<THREADS>(pref, e, D8_COST, cut.head);
+  const uint32_t mul = p.block_idx ? 1 : p.Hkv;
+  uint32_t rem = e - (static_cast<uint32_t>(pref[lo].x) * D8_COST + static_cast<uint32_t>(pref[lo].y) * cut.head), cnt;
+  int first = pref[lo].x;
+  if (per == 1) {
+    cnt = static_cast<uint32_t>(pref[lo + 1].x - first) / mul;
+  } else {
+    int u = lo * per;
+    for (cnt = d8_count(p, u); rem >= mul * (cnt ? cnt * D8_COST + cut.head : 0); cnt = d8_count(p, ++u)) {
+      rem -= mul * (cnt ? cnt * D8_COST + cut.head : 0);
+      first += static_cast<int>(mul * cnt);
+    }
+  }
+  const uint32_t one = cnt * D8_COST + cut.head, h = rem / one;
+  return first + static_cast<int>(h * cnt + cut.block(rem - h * one));
+}
+// Block x of the list, for a warp whose first lane asks for block x0 <= x.
+template <int THREADS>
+__device__ __forceinline__ D8Item d8_item(const kvskip_decode8_params& p, const int2* pref, const int per, const int x0, const int x) {
   D8Item it;
-  int lo = 0, hi = THREADS - 1;          // last t with pref[t] <= x
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (pref[mid] <= x) lo = mid; else hi = mid - 1;
+  int lo = d8_find<THREADS>(pref, x0, 1, 0);
+  if (pref[lo + 1].x <= x) {             // behind that share: the last t with pref[t].x <= x
+    int hi = THREADS - 1;
+    ++lo;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pref[mid].x <= x) lo = mid; else hi = mid - 1;
+    }
   }
   const uint32_t Hkv = p.Hkv;
   const int mul = p.block_idx ? 1 : p.Hkv;
-  int rem = x - pref[lo], u = lo, cnt;
+  int rem = x - pref[lo].x, u = lo, cnt;
   if (per == 1) {
-    cnt = pref[lo + 1] - pref[lo];
+    cnt = pref[lo + 1].x - pref[lo].x;
     if (!p.block_idx) cnt = static_cast<int>(static_cast<uint32_t>(cnt) / Hkv);
   } else {
     u = lo * per, cnt = d8_count(p, u);
@@ -235,8 +281,8 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[NW * 2];
-  __shared__ int pref[NT + 1];
-  __shared__ int wsum[NW];
+  __shared__ int2 pref[NT + 1];
+  __shared__ int2 wsum[NW];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.Hq / p.Hkv;
@@ -255,46 +301,60 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
     const int64_t at = (static_cast<int64_t>(blockIdx.x) * NT + tid) * 32;
     if (at < static_cast<int64_t>(p.B) * p.max_pages) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.page_table + at));
   }
-  // ---- the work list: items before every thread's share of the units, and all of them
+  // ---- the work list: blocks and heads before every thread's share of the units, and all of them
   const int units = p.block_idx ? p.B * p.Hkv : p.B;
   const int mul = p.block_idx ? 1 : p.Hkv;
   const int per = (units + NT - 1) / NT;
-  int mine = 0;
-  for (int u = tid * per; u < min(units, (tid + 1) * per); ++u) mine += d8_count(p, u) * mul;
-  int incl = mine;
+  int2 mine = make_int2(0, 0);
+  for (int u = tid * per; u < min(units, (tid + 1) * per); ++u) {
+    const int n = d8_count(p, u);
+    mine.x += n * mul, mine.y += n ? mul : 0;
+  }
+  int2 incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
+    const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+    if (lane >= o) incl.x += x, incl.y += y;
   }
   if (lane == 31) wsum[warp] = incl;
   __syncthreads();
-  int before = 0, W = 0;
+  int2 before = make_int2(0, 0), total = make_int2(0, 0);
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
-    if (w < warp) before += wsum[w];
-    W += wsum[w];
+    const int2 t = wsum[w];
+    if (w < warp) before.x += t.x, before.y += t.y;
+    total.x += t.x, total.y += t.y;
   }
-  pref[tid] = before + incl - mine;
-  if (tid == 0) pref[NT] = W;
+  pref[tid] = make_int2(before.x + incl.x - mine.x, before.y + incl.y - mine.y);
+  if (tid == 0) pref[NT] = total;
   __syncthreads();
 
   int* counter = static_cast<int*>(p.work);
   float* pieces = static_cast<float*>(p.work) + d8_piece_base(units);
-  const D8Chunks cut(W, NW * gridDim.x, shared);
-  if (blockIdx.x == 0) {                 // for the join: items before every unit
-    int x = pref[tid];
+  const D8Chunks cut(total.x, total.y, NW * gridDim.x, shared);
+  if (blockIdx.x == 0) {                 // for the join: blocks and heads before every unit
+    int2* out = reinterpret_cast<int2*>(counter + 4);
+    int2 x = pref[tid];
     for (int u = tid * per; u < min(units, (tid + 1) * per); ++u) {
-      counter[4 + u] = x;
-      if (per > 1) x += d8_count(p, u) * mul;
+      out[u] = x;
+      if (per > 1) {
+        const int n = d8_count(p, u);
+        x.x += n * mul, x.y += n ? mul : 0;
+      }
     }
-    if (tid == 0) counter[4 + units] = W;
+    if (tid == 0) out[units] = total;
   }
+  // the blocks [from, to) of chunk i, and 32 of them in the lanes
+  auto range = [&](const uint32_t i, int& from, int& to) {
+    from = d8_first<NT>(p, cut, pref, per, cut.edge(i));
+    to = d8_first<NT>(p, cut, pref, per, cut.edge(i + 1));
+  };
+  auto items = [&](const int from, const int n) { return d8_item<NT>(p, pref, per, from, from + min(lane, n - 1)); };
 
   // neighbouring chunks on different SMs: a short list spreads over all of them
   int chunk = warp * gridDim.x + blockIdx.x;
   int begin = 0, end = 0;                // what is left of the chunk
-  if (static_cast<uint32_t>(chunk) < cut.na) cut.range(chunk, begin, end);
+  if (static_cast<uint32_t>(chunk) < cut.na) range(chunk, begin, end);
 
   if (begin < end) {
     unsigned char* kstage = smem + warp * 2 * Cfg::kTile;
@@ -305,7 +365,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
     // up to 32 items of a chunk are in the lanes of `now`, the ones behind them (of the next chunk, at its end) in `next`
     int n = min(32, end - begin);
     int next_n = 0, next_begin = 0, next_end = end, next_chunk = chunk;
-    D8Item now = d8_item<NT>(p, pref, per, begin + min(lane, n - 1)), next = now;
+    D8Item now = items(begin, n), next = now;
 
     int64_t cur = -1;                    // first row of q of the head the warp is in
     auto load = [&](const D8Item& from, const int i, const bool is_v) {
@@ -381,7 +441,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
       if (li == 0 && !tail) {
         next_begin = begin + n;
         next_n = min(32, end - next_begin);
-        next = d8_item<NT>(p, pref, per, next_begin + min(lane, next_n - 1));
+        next = items(next_begin, next_n);
       }
       if (tail && cut.nb) {                        // take a chunk, one item ahead of its first load
         if (li == max(0, n - 2) && lane == 0) taken = atomicAdd(counter, 1);
@@ -389,9 +449,9 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
           const uint32_t got = cut.na + __shfl_sync(0xffffffffu, taken, 0);
           if (got < cut.count()) {
             next_chunk = static_cast<int>(got);
-            cut.range(got, next_begin, next_end);
+            range(got, next_begin, next_end);
             next_n = min(32, next_end - next_begin);
-            next = d8_item<NT>(p, pref, per, next_begin + min(lane, next_n - 1));
+            next = items(next_begin, next_n);
           }
         }
       }
@@ -658,44 +718,47 @@ decode8_merge_kernel(const __grid_constant__ kvskip_decode8_params p, const int 
   constexpr int COLS = Cfg::kCols, L = D / 4, NT = D8_MERGE_THREADS;
   __shared__ float4 sx[NT];
   __shared__ float sl[NT], sm[NT];
-  __shared__ int wsum[NT / 32], span[2];
+  __shared__ int2 wsum[NT / 32], span[2];
   const int bh = blockIdx.x, G = p.Hq / p.Hkv, tid = threadIdx.x, lane = tid & 31;
   const int units = p.block_idx ? p.B * p.Hkv : p.B;
-  const int* pref = static_cast<const int*>(p.work) + 4;
-  const int b = bh / p.Hkv, u = p.block_idx ? bh : b;
-  int first, count, W;
+  const int b = bh / p.Hkv, u = p.block_idx ? bh : b, mul = p.block_idx ? 1 : p.Hkv;
+  int2 first, next, total;               // blocks and heads before the unit, behind it, in all
   if (units <= NT) {
     // Before the wait: the lengths are older than the kernel this one waits for (which let this one begin only after
     // its own wait), so the place of the head in the list can be had while that one is at work.
-    const int mine = tid < units ? d8_count(p, tid) * (p.block_idx ? 1 : p.Hkv) : 0;
-    int incl = mine;
+    const int n = tid < units ? d8_count(p, tid) : 0;
+    int2 incl = make_int2(n * mul, n ? mul : 0);
+    const int2 mine = incl;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+      if (lane >= o) incl.x += x, incl.y += y;
     }
     if (lane == 31) wsum[tid >> 5] = incl;
     __syncthreads();
-    W = 0;
+    total = make_int2(0, 0);
 #pragma unroll
     for (int w = 0; w < NT / 32; ++w) {
-      if (w < (tid >> 5)) incl += wsum[w];
-      W += wsum[w];
+      const int2 t = wsum[w];
+      if (w < (tid >> 5)) incl.x += t.x, incl.y += t.y;
+      total.x += t.x, total.y += t.y;
     }
-    if (tid == u) span[0] = incl - mine, span[1] = mine;
+    if (tid == u) span[0] = make_int2(incl.x - mine.x, incl.y - mine.y), span[1] = incl;
     __syncthreads();
-    first = span[0], count = span[1];
+    first = span[0], next = span[1];
   } else {
     pdl_wait_prior();
-    first = pref[u], count = pref[u + 1] - first, W = pref[units];
+    const int2* pref = reinterpret_cast<const int2*>(static_cast<const int*>(p.work) + 4);
+    first = pref[u], next = pref[u + 1], total = pref[units];
   }
-  if (!p.block_idx) {
-    count = static_cast<int>(static_cast<uint32_t>(count) / static_cast<uint32_t>(p.Hkv));
-    first += (bh - b * p.Hkv) * count;
-  }
-  const D8Chunks cut(W, warps, shared);
+  const uint32_t count = static_cast<uint32_t>(next.x - first.x) / static_cast<uint32_t>(mul);
+  const D8Chunks cut(total.x, total.y, warps, shared);
   int c0 = 0, c1 = 0;
-  if (count) c0 = static_cast<int>(cut.of(first)), c1 = static_cast<int>(cut.of(first + count - 1));
+  if (count) {
+    const uint32_t h = p.block_idx ? 0 : bh - b * p.Hkv;
+    const uint32_t at = static_cast<uint32_t>(first.x) * D8_COST + static_cast<uint32_t>(first.y) * cut.head + h * (count * D8_COST + cut.head);
+    c0 = static_cast<int>(cut.of(at)), c1 = static_cast<int>(cut.of(at + cut.at(count - 1)));
+  }
   pdl_wait_prior();
   pdl_launch_dependents();
   const int64_t hq0 = static_cast<int64_t>(b) * p.Hq + (bh - b * p.Hkv) * G;

@@ -59,7 +59,7 @@ def _decode_params(**kw):
     (dict(page_table=4096, max_pages=1, num_pages=9), b"page table"), (dict(page_table=4096, max_pages=2), b"page table"),
     (dict(page_table=4096, max_pages=2, num_pages=9, lens=0), b"needs lens"), (dict(q=4100), b"8-byte"),
     (dict(q_sh=130), b"8-byte"), (dict(k=4104), b"16-byte"), (dict(v_st=136), b"16"), (dict(work=4100), b"misaligned"),
-    (dict(B=1 << 20, T=1 << 20, nb=1 << 14), b"2^31")])
+    (dict(B=1 << 20, T=1 << 20, nb=1 << 14), b"2^29")])
 def test_decode8_entry_refuses(lib, change, text):
     assert lib.kvskip_launch_decode8(ctypes.byref(_decode_params(**change)), None) < 0
     assert text in lib.kvskip_last_error()
