@@ -96,7 +96,7 @@ int launch_decode8(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cuda
   KVB_CUDA(launch(kernel, dim3(l.ctas), Cfg::kThreads, Cfg::kSmem, stream, p, maps, l.shared));
   // few heads: the output of one goes to several blocks, of 8 quads at least
   const int quads = p.Hq / p.Hkv * D / 4, heads = p.B * p.Hkv;
-  const int y = std::max(1, std::min(quads / 8, 4 * kvb_host::num_sms() / heads));
+  const int y = std::max(1, std::min(quads / 8, 2 * kvb_host::num_sms() / heads));
   KVB_CUDA(launch(kvb::decode8_merge_kernel<D, MODE>, dim3(heads, y), kvb::D8_MERGE_THREADS, 0, stream, p, l.warps, l.shared));
   return KVSKIP_OK;
 }

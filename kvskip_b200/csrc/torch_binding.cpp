@@ -751,6 +751,31 @@ int check_cache8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
 at::Tensor new_cuda(at::IntArrayRef shape, at::ScalarType type, const at::Device& device) {
   return at::detail::empty_cuda(shape, type, device, c10::nullopt);
 }
+// Several tensors in one allocation (each 256-byte aligned): one trip to the allocator instead of one per tensor.
+struct NewTogether {
+  std::vector<std::pair<at::Tensor*, std::pair<c10::SmallVector<int64_t, 2>, at::ScalarType>>> parts;
+  void add(at::Tensor& t, at::IntArrayRef shape, at::ScalarType type) {
+    parts.push_back({&t, {c10::SmallVector<int64_t, 2>(shape.begin(), shape.end()), type}});
+  }
+  void make(const at::Device& device) {
+    const auto bytes = [](const c10::SmallVector<int64_t, 2>& shape, const at::ScalarType type) {
+      int64_t n = static_cast<int64_t>(c10::elementSize(type));
+      for (const int64_t d : shape) n *= d;
+      return (n + 255) / 256 * 256;
+    };
+    int64_t total = 0;
+    for (const auto& p : parts) total += bytes(p.second.first, p.second.second);
+    const at::Tensor all = new_cuda({total}, at::kByte, device);
+    int64_t at_byte = 0;
+    for (const auto& p : parts) {
+      const at::ScalarType type = p.second.second;
+      *p.first = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+      p.first->unsafeGetTensorImpl()->set_storage_offset(at_byte / static_cast<int64_t>(c10::elementSize(type)));
+      p.first->unsafeGetTensorImpl()->set_sizes_contiguous(p.second.first);
+      at_byte += bytes(p.second.first, type);
+    }
+  }
+};
 // whether every front-end call is to check the status word (the variable may change while the process runs)
 bool check_wanted() {
   const char* e = std::getenv("KVSKIP_CHECK_STATUS");
@@ -891,7 +916,7 @@ void write8(const at::Tensor& k_new, const at::Tensor& v_new, const at::Tensor& 
 
 void fill_pages(kvskip_pages_params& p, const at::Tensor& lens, const at::Tensor& page_table, const at::Tensor& free_pages,
                 const at::Tensor& n_free, const c10::optional<at::Tensor>& lens_out,
-                const c10::optional<at::Tensor>& n_free_out, at::Tensor& lo, at::Tensor& fo) {
+                const c10::optional<at::Tensor>& n_free_out, at::Tensor& lo, at::Tensor& fo, NewTogether& fresh) {
   p.lens = i32(lens, "lens");
   i32(page_table, "page_table");
   i32(free_pages, "free_pages");
@@ -900,8 +925,11 @@ void fill_pages(kvskip_pages_params& p, const at::Tensor& lens, const at::Tensor
                   page_table.size(1) >= 1, "lens: [B], page_table: [B, max_pages]");
   TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) >= 1 && n_free.numel() == 1, "free_pages: [pages], n_free: one element");
   same_device(lens, {&page_table, &free_pages, &n_free});
-  lo = lens_out.has_value() ? *lens_out : new_cuda(lens.sizes(), at::kInt, lens.device());
-  fo = n_free_out.has_value() ? *n_free_out : new_cuda(n_free.sizes(), at::kInt, lens.device());
+  if (lens_out.has_value()) lo = *lens_out;
+  else fresh.add(lo, lens.sizes(), at::kInt);
+  if (n_free_out.has_value()) fo = *n_free_out;
+  else fresh.add(fo, n_free.sizes(), at::kInt);
+  fresh.make(lens.device());
   p.lens_out = const_cast<int32_t*>(i32(lo, "lens_out"));
   p.n_free_out = const_cast<int32_t*>(i32(fo, "n_free_out"));
   TORCH_CHECK(lo.numel() == lens.numel() && fo.numel() == 1, "lens_out: [B], n_free_out: one element");
@@ -920,21 +948,22 @@ std::vector<at::Tensor> extend_pages(const at::Tensor& lens, const at::Tensor& n
                                      const c10::optional<at::Tensor>& n_free_out) {
   TORCH_CHECK(lens.is_cuda(), "lens: contiguous CUDA int32");
   const c10::cuda::CUDAGuard guard(lens.device());
-  kvskip_pages_params p{};
-  at::Tensor lo, fo;
-  fill_pages(p, lens, page_table, free_pages, n_free, lens_out, n_free_out, lo, fo);
-  p.new_ = i32(new_, "new");
-  TORCH_CHECK(new_.numel() == lens.numel(), "new: [B]");
-  same_device(lens, {&new_});
+  TORCH_CHECK(lens.dim() == 1 && new_.numel() == lens.numel(), "new: [B]");
   const int64_t B = lens.size(0);
   TORCH_CHECK(per_row >= 0 && n_tokens >= 0 && (per_row == 0 || per_row <= std::numeric_limits<int32_t>::max()),
               "extend_pages: n_tokens or per_row");
   const int64_t n = per_row ? B * per_row : n_tokens;
   const int64_t dims[2] = {per_row ? B : n, per_row};
   const at::IntArrayRef shape(dims, per_row ? 2 : 1);
-  at::Tensor slots = new_cuda(shape, at::kLong, lens.device());
-  at::Tensor positions = new_cuda(shape, at::kInt, lens.device());
-  at::Tensor granted = new_cuda({B}, at::kBool, lens.device());
+  kvskip_pages_params p{};
+  at::Tensor lo, fo, slots, positions, granted;
+  NewTogether fresh;
+  fresh.add(slots, shape, at::kLong);
+  fresh.add(positions, shape, at::kInt);
+  fresh.add(granted, {B}, at::kBool);
+  fill_pages(p, lens, page_table, free_pages, n_free, lens_out, n_free_out, lo, fo, fresh);
+  p.new_ = i32(new_, "new");
+  same_device(lens, {&new_});
   p.slots = slots.data_ptr<int64_t>();
   p.positions = positions.data_ptr<int32_t>();
   p.granted = static_cast<uint8_t*>(granted.data_ptr());
@@ -955,7 +984,8 @@ std::vector<at::Tensor> release_pages(const at::Tensor& done, const at::Tensor& 
   const c10::cuda::CUDAGuard guard(lens.device());
   kvskip_pages_params p{};
   at::Tensor lo, fo;
-  fill_pages(p, lens, page_table, free_pages, n_free, lens_out, n_free_out, lo, fo);
+  NewTogether fresh;
+  fill_pages(p, lens, page_table, free_pages, n_free, lens_out, n_free_out, lo, fo, fresh);
   same_device(lens, {&done});
   p.done = u8(done);
   raise_on(kvskip_launch_release_pages(&p, cur_stream()));
