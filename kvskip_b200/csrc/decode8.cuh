@@ -693,8 +693,10 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
       phase ^= 1;
 
       const bool ends = (info >> 9) & 1;
-      if (ends || (last && tail)) flush(ends);
-      if (ends) cur = -1;
+      if (ends || (last && tail)) {
+        flush(ends);
+        cur = -1;                        // (a next chunk of the same head is a piece of its own; its q is still in place)
+      }
       if (!last) {
         ++li;
         continue;

@@ -158,6 +158,48 @@ def test_decode8_block_lists(kind, layout, G):
     _check(_run(d, plan=K.Plan(idx, plan.block_cnt, nb, nb), stats=True), ref, D, nb, torch.bfloat16)
 
 
+@pytest.mark.parametrize("Hkv,T,masked", [(1, 45000 * 64 - 11, False), (2, 23000 * 64, True)])
+def test_decode8_chunks_taken_from_the_counter(Hkv, T, masked):
+    """Enough blocks per warp for the shared part of the work list, in so few heads that every warp takes several chunks
+    of the same one.  The 64-bit sums are formed on the GPU, a stretch of the sequence at a time."""
+    D, G, B = 64, 4, 1
+    gen = torch.Generator(device=DEV).manual_seed(T)
+    nb = -(-T // TILE)
+    k, v = (torch.randint(-127, 128, (B, Hkv, T, D), generator=gen, device=DEV, dtype=torch.int8) for _ in range(2))
+    ks, vs = (torch.exp(0.3 * torch.randn(B, Hkv, nb, generator=gen, device=DEV)) / 70 for _ in range(2))
+    q = torch.randn(B, Hkv * G, D, generator=gen, device=DEV).to(torch.float16)
+    scale, plan = 1 / math.sqrt(D), None
+    keep = torch.ones(Hkv, nb, dtype=torch.bool, device=DEV)
+    if masked:
+        keep = torch.rand(Hkv, nb, generator=gen, device=DEV) < 0.98
+        plan = K.make_plan(keep[None])
+    r = K.decode8(q, k, v, ks, vs, scale, plan=plan, out_f32=True)
+    out = {n: torch.zeros(B, Hkv * G, D, dtype=torch.float64) for n in ("out", "mag")}
+    lse, qk = torch.zeros(B, Hkv * G, dtype=torch.float64), torch.zeros(B, Hkv * G, dtype=torch.float64)
+    for h in range(Hkv):
+        qh = q[0, h * G:(h + 1) * G].double()
+        rows, parts = slice(h * G, (h + 1) * G), []
+        for t0 in range(0, T, 1 << 18):
+            t1 = min(T, t0 + (1 << 18))
+            blk = torch.arange(t0, t1, device=DEV) // TILE
+            kk, vv = k[0, h, t0:t1].double() * ks[0, h, blk].double()[:, None], v[0, h, t0:t1].double() * vs[0, h, blk].double()[:, None]
+            s = (qh @ kk.T * scale).masked_fill(~keep[h, blk], -math.inf)
+            m = s.amax(1, keepdim=True)
+            p = torch.exp(s - m)
+            parts.append((m, p.sum(1, keepdim=True), p @ vv, p @ vv.abs(), (qh.abs() @ kk.abs().T).amax(1) * scale))
+        top = torch.cat([x[0] for x in parts], 1).amax(1, keepdim=True)
+        w = [torch.exp(x[0] - top) for x in parts]
+        total = sum(x[1] * f for x, f in zip(parts, w))
+        out["out"][0, rows] = (sum(x[2] * f for x, f in zip(parts, w)) / total).cpu()
+        out["mag"][0, rows] = (sum(x[3] * f for x, f in zip(parts, w)) / total).cpu()
+        lse[0, rows] = (top + torch.log(total))[:, 0].cpu()
+        qk[0, rows] = torch.stack([x[4] for x in parts]).amax(0).cpu()
+    # (the sums run over a warp's chunks, then over the pieces: far fewer than nb additions one after the other)
+    _check(r, {**out, "lse": lse, "qk": qk}, D, nb, torch.float16)
+    again = K.decode8(q, k, v, ks, vs, scale, plan=plan, out_f32=True)
+    assert torch.equal(again["out_f32"], r["out_f32"]) and torch.equal(again["lse"], r["lse"])
+
+
 def test_decode8_strides_and_optional_lengths():
     B, Hkv, G, D, T = 2, 4, 4, 128, 333
     c = _case([T] * B, Hkv, G, D, "e4m3", torch.bfloat16, "contiguous", seed=9)
