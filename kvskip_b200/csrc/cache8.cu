@@ -25,18 +25,27 @@ using kvb_host::fail;
 
 // Programmatic dependent launch: every kernel here waits for its predecessor before it touches global memory.
 template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
+cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, unsigned cluster, size_t smem, cudaStream_t stream,
+                           Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = kvb_host::use_pdl() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
+  return launch_cluster(kernel, grid, threads, 0, smem, stream, static_cast<Args&&>(args)...);
 }
 
 bool misaligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
@@ -67,37 +76,60 @@ int make_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int6
 
 // What of a launch follows from the bound on its items (the lengths are on the device).
 struct Decode8Launch {
-  int ctas, warps, shared;
+  int ctas, warps, cluster;            // cluster: CTAs per head of the short form, 0 where that is not taken
 };
+// Blocks per warp up to which the short form is taken when its CTAs are most of the SMs, and when they are fewer.  The
+// lengths are on the device: with one bound on them for all, a longer form would leave SMs idle when they differ.
+// B200, us, general and short form, D 128, 8 KV heads: batch 1 / 1k 9.2 and 8.1, 4k 9.6 and 8.7, 8k 10.4 and 11.0; batch 4 / 4k
+// 13.7 and 11.6, batch 16 / 2k 19.5 and 16.5.
+constexpr int kShortMost = 4, kShortFew = 2;
 template <int D, int MODE>
 Decode8Launch decode8_launch(const kvskip_decode8_params& p) {
   const int64_t items = static_cast<int64_t>(p.B) * p.Hkv * (p.block_idx ? p.max_blocks : p.nb);
   Decode8Launch l;
   l.ctas = static_cast<int>(std::min<int64_t>(kvb_host::num_sms(), items));
   l.warps = l.ctas * kvb::D8Cfg<D, MODE>::kWarps;
-  l.shared = items >= kvb::D8_SHARE_MIN * static_cast<int64_t>(l.warps);
+  // the short form: as many CTAs per head as give every block a warp, in one wave
+  const int64_t heads = static_cast<int64_t>(p.B) * p.Hkv, longest = p.block_idx ? p.max_blocks : p.nb;
+  int c = 1;
+  while (c < 8 && c * kvb::D8Cfg<D, MODE>::kWarps < longest && heads * 2 * c <= kvb_host::num_sms()) c *= 2;
+  const bool most = 4 * heads * c >= 3 * kvb_host::num_sms();
+  l.cluster = 0;
+  // (not for more than 8 query heads: the pieces are four times as large, and joining them so took longer)
+  if (MODE < 2 && heads * c <= kvb_host::num_sms() &&
+      longest <= static_cast<int64_t>(most ? kShortMost : kShortFew) * c * kvb::D8Cfg<D, MODE>::kWarps)
+    l.cluster = c;
   return l;
 }
 template <int D, int MODE>
 int64_t decode8_work(const kvskip_decode8_params& p) {
   const Decode8Launch l = decode8_launch<D, MODE>(p);
+  if (l.cluster) return 16;
   const int64_t units = p.block_idx ? static_cast<int64_t>(p.B) * p.Hkv : p.B;
-  return (kvb::d8_piece_base(units) + (l.shared ? 4 : 1) * 2 * static_cast<int64_t>(l.warps) * kvb::D8Cfg<D, MODE>::kPiece) *
+  return (kvb::d8_piece_base(units) + 2 * static_cast<int64_t>(l.warps) * kvb::D8Cfg<D, MODE>::kPiece) *
          static_cast<int64_t>(sizeof(float));
 }
 
 template <int KIND, int D, int MODE>
 int launch_decode8(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cudaStream_t stream) {
   using Cfg = kvb::D8Cfg<D, MODE>;
-  auto kernel = kvb::decode8_kernel<KIND, D, MODE>;
-  if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmem)) return rc;
   const Decode8Launch l = decode8_launch<D, MODE>(p);
-  if (l.shared) KVB_CUDA(launch(kvb::decode8_begin_kernel, dim3(1), 1, 0, stream, static_cast<int*>(p.work)));
-  KVB_CUDA(launch(kernel, dim3(l.ctas), Cfg::kThreads, Cfg::kSmem, stream, p, maps, l.shared));
+  if constexpr (MODE < 2) {
+    if (l.cluster) {
+      auto kernel = kvb::decode8_kernel<KIND, D, MODE, true>;
+      if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmem)) return rc;
+      KVB_CUDA(launch_cluster(kernel, dim3(static_cast<unsigned>(p.B) * p.Hkv * l.cluster), Cfg::kThreads,
+                              static_cast<unsigned>(l.cluster), Cfg::kSmem, stream, p, maps));
+      return KVSKIP_OK;
+    }
+  }
+  auto kernel = kvb::decode8_kernel<KIND, D, MODE, false>;
+  if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmem)) return rc;
+  KVB_CUDA(launch(kernel, dim3(l.ctas), Cfg::kThreads, Cfg::kSmem, stream, p, maps));
   // few heads: the output of one goes to several blocks, of 8 quads at least
   const int quads = p.Hq / p.Hkv * D / 4, heads = p.B * p.Hkv;
   const int y = std::max(1, std::min(quads / 8, 2 * kvb_host::num_sms() / heads));
-  KVB_CUDA(launch(kvb::decode8_merge_kernel<D, MODE>, dim3(heads, y), kvb::D8_MERGE_THREADS, 0, stream, p, l.warps, l.shared));
+  KVB_CUDA(launch(kvb::decode8_merge_kernel<D, MODE>, dim3(heads, y), kvb::D8_MERGE_THREADS, 0, stream, p, l.warps));
   return KVSKIP_OK;
 }
 

@@ -11,13 +11,14 @@
 // written back there first, which costs more than the products do.
 //
 // Work split: the (sequence, head, block) items of the whole launch are one list, ordered by sequence,
-// head and block, cut into chunks; a warp takes one chunk after the other.  So requests of any mixture of
-// lengths keep every SM busy to the end without the host knowing a length.  A warp keeps the running maximum, sum
+// head and block, cut evenly into one chunk per warp.  So requests of any mixture of lengths keep every SM busy to the end
+// without the host knowing a length.  A warp keeps the running maximum, sum
 // and output of the head it is in and has its own stage (a K and a V tile with an mbarrier each, refilled as soon as
 // its products are done): no barrier between warps anywhere.  A head that a chunk holds from its first to its last
 // block is written out by the warp; other pieces (at most two per chunk) go to `work` and are joined, in item order,
-// by decode8_merge_kernel.  Where the chunks begin depends on the list alone, not on who takes them: results do not
-// depend on timing.
+// by decode8_merge_kernel.  Nothing is added in an order that depends on timing.  (Chunks taken from a counter, so that SMs
+// which get less of a saturated memory do less, gained nothing: with 8 warps an SM the SMs finish within a few
+// per cent of each other, with 12 they differed by a third.)
 //
 // P (0..1 relative to its block's maximum) goes to the tensor cores as fp16 high + low parts, which hold
 // 22 bits of it: with G <= 4 the two parts share one instruction (columns 0-3 high, 4-7 low; the scores of a
@@ -53,48 +54,29 @@ constexpr float D8_PSCALE = 13.f;   // log2 of the scaling of P
 // average) and a warp has at least four blocks, the first block of a head D8_HEAD more (q is read and converted there, and
 // the output written at the end: 2.7 us per block of a long head, 3.7 us per head of one block, measured with every warp
 // of a B200 at work; a ragged batch of 64 takes 45 us with it, 50 without).  A block belongs to the chunk in which it
-// begins.  Every warp has one chunk to begin with.  Under a saturated memory SMs differ in the bandwidth
-// they get (by their place on the die), so with enough blocks per warp the first chunks are five eighths of the list
-// only; two eighths are cut into one more chunk per warp and the last eighth into two, which the warps take from a
-// counter as they get there (batch 16 / 64k: 335 -> 318 us; with 11 blocks per warp it costs more than it gives).
+// begins; every chunk is at least as long as the longest block, so none is empty.
 constexpr int D8_COST = 4, D8_HEAD = 2;
 constexpr int D8_HEAD_MIN = 4;       // blocks per warp from which on heads are counted,
 constexpr int D8_HEAD_MAX = 64;      // and the mean length of a head up to which they are
-constexpr int D8_SHARE_MIN = 24;     // blocks per warp from which on chunks are taken from the counter
-struct D8Zone {                      // costs from `base` on, cut into the chunks from `first` on: the first `longer` of
-  uint32_t base, first, size, longer;   // them have size + 1, the others size
-  __device__ __forceinline__ D8Zone(uint32_t base_, uint32_t costs, uint32_t first_, uint32_t chunks)
-      : base(base_), first(first_), size(chunks ? costs / chunks : 0), longer(costs - size * chunks) {}
-  __device__ __forceinline__ uint32_t edge(const uint32_t i) const { return base + size * (i - first) + min(i - first, longer); }
-  __device__ __forceinline__ uint32_t of(uint32_t x) const {
-    x -= base;
-    const uint32_t split = longer * (size + 1);
-    return first + (x < split ? x / (size + 1) : longer + (x - split) / size);
-  }
-};
-// W blocks in `heads` heads.  Every chunk is at least as long as the longest block, so none is empty.
 struct D8Chunks {
   uint32_t head, all;                // cost of a head's beginning, of everything
-  uint32_t wb, wc, na, nb, nc;       // costs and chunks of the shared zones
-  D8Zone a, b, c;
-  __device__ __forceinline__ D8Chunks(const uint32_t W, const uint32_t heads, const uint32_t warps, const bool counter)
+  uint32_t count, size, longer;      // chunks; the first `longer` of them have cost size + 1, the others size
+  __device__ __forceinline__ D8Chunks(const uint32_t W, const uint32_t heads, const uint32_t warps)
       : head(W / D8_HEAD_MIN >= warps && W / D8_HEAD_MAX < heads ? D8_HEAD : 0), all(W * D8_COST + heads * head),
-        wb(counter && W / D8_SHARE_MIN >= warps ? all / 4 : 0), wc(wb / 2), na(min(W, warps)),
-        nb(min(wb / (3 * D8_COST), warps)), nc(min(wc / (3 * D8_COST), 2 * warps)),
-        a(0, all - wb - wc, 0, na), b(all - wb - wc, wb, na, nb), c(all - wc, wc, na + nb, nc) {}
-  __device__ __forceinline__ uint32_t count() const { return na + nb + nc; }
-  __device__ __forceinline__ uint32_t edge(const uint32_t i) const {       // where chunk i begins; i <= count()
-    return i < b.first ? a.edge(i) : i < c.first ? b.edge(i) : nc ? c.edge(i) : all;
+        count(min(W, warps)), size(count ? all / count : 0), longer(all - size * count) {}
+  __device__ __forceinline__ uint32_t edge(const uint32_t i) const { return size * i + min(i, longer); }
+  __device__ __forceinline__ uint32_t of(const uint32_t x) const {
+    const uint32_t split = longer * (size + 1);
+    return x < split ? x / (size + 1) : longer + (x - split) / size;
   }
-  __device__ __forceinline__ uint32_t of(const uint32_t x) const { return x < b.base ? a.of(x) : x < c.base ? b.of(x) : c.of(x); }
   // first cost of block j of a head, and the first block that begins at or behind cost r of one
   __device__ __forceinline__ uint32_t at(const uint32_t j) const { return j ? head + j * D8_COST : 0; }
   __device__ __forceinline__ uint32_t block(const uint32_t r) const {
     return r == 0 ? 0 : r <= head + D8_COST ? 1 : (r - head + D8_COST - 1) / D8_COST;
   }
 };
-// Layout of `work`: [0] the counter, [4..] blocks and heads before every unit of the list, then the pieces (two per chunk).
-__host__ __device__ inline int64_t d8_piece_base(const int64_t units) { return (4 + 2 * (units + 1) + 3) / 4 * 4; }
+// Layout of `work`: blocks and heads before every unit of the list, then the pieces (two per chunk).
+__host__ __device__ inline int64_t d8_piece_base(const int64_t units) { return (2 * (units + 1) + 3) / 4 * 4; }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -184,40 +166,10 @@ __device__ __forceinline__ int d8_first(const kvskip_decode8_params& p, const D8
   const uint32_t one = cnt * D8_COST + cut.head, h = rem / one;
   return first + static_cast<int>(h * cnt + cut.block(rem - h * one));
 }
-// Block x of the list, for a warp whose first lane asks for block x0 <= x.
-template <int THREADS>
-__device__ __forceinline__ D8Item d8_item(const kvskip_decode8_params& p, const int2* pref, const int per, const int x0, const int x) {
+// Block number j of the cnt blocks of KV head h of sequence b.
+__device__ __forceinline__ D8Item d8_block(const kvskip_decode8_params& p, const int b, const int h, const int j, const int cnt) {
   D8Item it;
-  int lo = d8_find<THREADS>(pref, x0, 1, 0);
-  if (pref[lo + 1].x <= x) {             // behind that share: the last t with pref[t].x <= x
-    int hi = THREADS - 1;
-    ++lo;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pref[mid].x <= x) lo = mid; else hi = mid - 1;
-    }
-  }
-  const uint32_t Hkv = p.Hkv;
-  const int mul = p.block_idx ? 1 : p.Hkv;
-  int rem = x - pref[lo].x, u = lo, cnt;
-  if (per == 1) {
-    cnt = pref[lo + 1].x - pref[lo].x;
-    if (!p.block_idx) cnt = static_cast<int>(static_cast<uint32_t>(cnt) / Hkv);
-  } else {
-    u = lo * per, cnt = d8_count(p, u);
-    while (rem >= cnt * mul) {
-      rem -= cnt * mul;
-      cnt = d8_count(p, ++u);
-    }
-  }
-  int b, h, j;
-  if (p.block_idx) {
-    b = static_cast<int>(static_cast<uint32_t>(u) / Hkv), h = u - b * p.Hkv, j = rem;
-    it.blk = p.block_idx[static_cast<int64_t>(u) * p.max_blocks + j];
-  } else {
-    b = u, h = static_cast<int>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(cnt)), j = rem - h * cnt;
-    it.blk = j;
-  }
+  it.blk = p.block_idx ? p.block_idx[(static_cast<int64_t>(b) * p.Hkv + h) * p.max_blocks + j] : j;
   it.b = b;
   const bool in = it.blk >= 0 && it.blk < p.nb;
   const int tok = in ? max(0, min(TILE, d8_len(p, b) - it.blk * TILE)) : 0;
@@ -244,6 +196,39 @@ __device__ __forceinline__ D8Item d8_item(const kvskip_decode8_params& p, const 
   return it;
 }
 
+// Block x of the list, for a warp whose first lane asks for block x0 <= x.
+template <int THREADS>
+__device__ __forceinline__ D8Item d8_item(const kvskip_decode8_params& p, const int2* pref, const int per, const int x0, const int x) {
+  int lo = d8_find<THREADS>(pref, x0, 1, 0);
+  if (pref[lo + 1].x <= x) {             // behind that share: the last t with pref[t].x <= x
+    int hi = THREADS - 1;
+    ++lo;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pref[mid].x <= x) lo = mid; else hi = mid - 1;
+    }
+  }
+  const uint32_t Hkv = p.Hkv;
+  const int mul = p.block_idx ? 1 : p.Hkv;
+  int rem = x - pref[lo].x, u = lo, cnt;
+  if (per == 1) {
+    cnt = pref[lo + 1].x - pref[lo].x;
+    if (!p.block_idx) cnt = static_cast<int>(static_cast<uint32_t>(cnt) / Hkv);
+  } else {
+    u = lo * per, cnt = d8_count(p, u);
+    while (rem >= cnt * mul) {
+      rem -= cnt * mul;
+      cnt = d8_count(p, ++u);
+    }
+  }
+  if (p.block_idx) {
+    const int b = static_cast<int>(static_cast<uint32_t>(u) / Hkv);
+    return d8_block(p, b, u - b * p.Hkv, rem, cnt);
+  }
+  const int h = static_cast<int>(static_cast<uint32_t>(rem) / static_cast<uint32_t>(cnt));
+  return d8_block(p, u, h, rem - h * cnt, cnt);
+}
+
 // Output rows: o[head][d0], [d0 + 1] of query head hq.
 __device__ __forceinline__ void d8_store(const kvskip_decode8_params& p, const int64_t hq, const int d0, float a, float b) {
   uint32_t w;
@@ -263,17 +248,53 @@ __device__ __forceinline__ float d8_lse(float m, float l) {
   return l == 0.f ? -INFINITY : (m + log2f(l) - D8_PSCALE) * LN2;   // (a NaN sum stays one)
 }
 __device__ __forceinline__ float d8_safe(float m) { return m == -INFINITY ? 0.f : m; }
-
-// Zeroes the counter of a launch whose warps share chunks.
-__global__ void decode8_begin_kernel(int* counter) {
-  pdl_wait_prior();
-  pdl_launch_dependents();
-  *counter = 0;
+// N pieces (maximum, sum, four channels) onto a sum relative to m_old, which becomes one relative to m.
+template <int N>
+__device__ __forceinline__ void d8_add(const float m_old, const float m, const float (&pm)[N], const float (&pl)[N],
+                                       const float4 (&v)[N], float& l, float4& x) {
+  const float mu = d8_safe(m), down = ex2(m_old - mu);
+  l *= down;
+  x.x *= down, x.y *= down, x.z *= down, x.w *= down;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float f = ex2(pm[i] - mu);
+    l += pl[i] * f;
+    x.x += v[i].x * f, x.y += v[i].y * f, x.z += v[i].z * f, x.w += v[i].w * f;
+  }
+}
+// The sums of S threads (every `quads`-th from `at` on), in order; m: the first one's maximum, then that of all.
+__device__ __forceinline__ void d8_join(const float4* sx, const float* sl, const float* sm, const int at, const int quads,
+                                        const int S, float& m, float& l, float4& x) {
+#pragma unroll 8
+  for (int i = 1; i < S; ++i) m = fmaxf(m, sm[i * quads + at]);
+  const float mu = d8_safe(m);
+  l = 0.f, x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int i = 0; i < S; ++i) {
+    const float f = ex2(sm[i * quads + at] - mu);
+    const float4 v = sx[i * quads + at];
+    l += sl[i * quads + at] * f;
+    x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
+  }
+}
+__device__ __forceinline__ float cluster_ld_f32(const uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_ld_f32x4(const uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 
-template <int KIND, int D, int MODE>
+// SHORT: the form for few short heads, a launch as short as it gets.  A cluster of CTAs takes one head, its warps the
+// head's blocks evenly; the pieces stay in shared memory and the CTAs of the cluster join a share of the output each,
+// reading the others' through distributed shared memory.  No list, no second launch.
+template <int KIND, int D, int MODE, bool SHORT>
 __global__ void __launch_bounds__(D8Cfg<D, MODE>::kThreads, 1)
-decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_constant__ D8Maps maps, const int shared) {
+decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_constant__ D8Maps maps) {
   using Cfg = D8Cfg<D, MODE>;
   constexpr int NW = Cfg::kWarps, NT = Cfg::kThreads, KS = D / 16;
   constexpr int CT = Cfg::kTiles, PT = Cfg::kParts, COLS = Cfg::kCols;
@@ -291,21 +312,38 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
     tma_prefetch_desc(&maps.k);
     tma_prefetch_desc(&maps.v);
   }
-  if (tid < NW * 2) mbar_init(&bars[tid], 1);
+  if (lane < 2) mbar_init(&bars[2 * warp + lane], 1);      // (a warp waits on its own barriers alone)
   mbar_fence_init();
+  __syncwarp();
   pdl_wait_prior();
   pdl_launch_dependents();
 
-  if (p.page_table) {
+  const int ranks = SHORT ? static_cast<int>(cluster_nctarank()) : 1, rank = SHORT ? static_cast<int>(cluster_ctarank()) : 0;
+  const int bh = SHORT ? blockIdx.x / ranks : 0, bs = bh / p.Hkv, hs = bh - bs * p.Hkv;   // SHORT: the cluster's head
+  const int cnt = SHORT ? d8_count(p, p.block_idx ? bh : bs) : 0;
+  if (SHORT && cnt == 0) {               // (the whole cluster leaves)
+    const int64_t hq0 = static_cast<int64_t>(bs) * p.Hq + hs * G;
+    if (rank) return;
+    for (int o = tid; o < G * (D / 4); o += NT) d8_store4(p, hq0 + o / (D / 4), 4 * (o % (D / 4)), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+    if (tid < G) p.lse[hq0 + tid] = -INFINITY;
+    if (p.blk_max)
+      for (int64_t o = tid; o < static_cast<int64_t>(G) * p.nb; o += NT) {
+        p.blk_max[hq0 * p.nb + o] = -INFINITY;
+        p.blk_sum[hq0 * p.nb + o] = 0.f;
+      }
+    return;
+  }
+  if (!SHORT && p.page_table) {
     // the page table into L2 while the lengths are on their way (128 bytes a thread cover 7 MB of it)
     const int64_t at = (static_cast<int64_t>(blockIdx.x) * NT + tid) * 32;
     if (at < static_cast<int64_t>(p.B) * p.max_pages) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.page_table + at));
   }
   // ---- the work list: blocks and heads before every thread's share of the units, and all of them
-  const int units = p.block_idx ? p.B * p.Hkv : p.B;
+  const int units = SHORT ? 0 : p.block_idx ? p.B * p.Hkv : p.B;
   const int mul = p.block_idx ? 1 : p.Hkv;
   const int per = (units + NT - 1) / NT;
-  int2 mine = make_int2(0, 0);
+  int2 mine = make_int2(0, 0), total = make_int2(0, 0);
+  if constexpr (!SHORT) {
   for (int u = tid * per; u < min(units, (tid + 1) * per); ++u) {
     const int n = d8_count(p, u);
     mine.x += n * mul, mine.y += n ? mul : 0;
@@ -318,7 +356,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
   }
   if (lane == 31) wsum[warp] = incl;
   __syncthreads();
-  int2 before = make_int2(0, 0), total = make_int2(0, 0);
+  int2 before = make_int2(0, 0);
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     const int2 t = wsum[w];
@@ -328,12 +366,12 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
   pref[tid] = make_int2(before.x + incl.x - mine.x, before.y + incl.y - mine.y);
   if (tid == 0) pref[NT] = total;
   __syncthreads();
+  }
 
-  int* counter = static_cast<int*>(p.work);
   float* pieces = static_cast<float*>(p.work) + d8_piece_base(units);
-  const D8Chunks cut(total.x, total.y, NW * gridDim.x, shared);
-  if (blockIdx.x == 0) {                 // for the join: blocks and heads before every unit
-    int2* out = reinterpret_cast<int2*>(counter + 4);
+  const D8Chunks cut(total.x, total.y, NW * gridDim.x);
+  if (!SHORT && blockIdx.x == 0) {       // for the join: blocks and heads before every unit
+    int2* out = static_cast<int2*>(p.work);
     int2 x = pref[tid];
     for (int u = tid * per; u < min(units, (tid + 1) * per); ++u) {
       out[u] = x;
@@ -344,17 +382,24 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
     }
     if (tid == 0) out[units] = total;
   }
-  // the blocks [from, to) of chunk i, and 32 of them in the lanes
-  auto range = [&](const uint32_t i, int& from, int& to) {
-    from = d8_first<NT>(p, cut, pref, per, cut.edge(i));
-    to = d8_first<NT>(p, cut, pref, per, cut.edge(i + 1));
+  // n blocks from `from` on in the lanes
+  auto items = [&](const int from, const int n) {
+    if constexpr (SHORT) return d8_block(p, bs, hs, from + min(lane, n - 1), cnt);
+    else return d8_item<NT>(p, pref, per, from, from + min(lane, n - 1));
   };
-  auto items = [&](const int from, const int n) { return d8_item<NT>(p, pref, per, from, from + min(lane, n - 1)); };
 
   // neighbouring chunks on different SMs: a short list spreads over all of them
-  int chunk = warp * gridDim.x + blockIdx.x;
-  int begin = 0, end = 0;                // what is left of the chunk
-  if (static_cast<uint32_t>(chunk) < cut.na) range(chunk, begin, end);
+  const int chunk = SHORT ? warp * ranks + rank : warp * gridDim.x + blockIdx.x;
+  int begin = 0, end = 0;                // what is left of it
+  if constexpr (SHORT) {
+    const int parts = NW * ranks, size = cnt / parts, longer = cnt - size * parts;
+    begin = chunk * size + min(chunk, longer), end = begin + size + (chunk < longer);
+  } else {
+    if (static_cast<uint32_t>(chunk) < cut.count) {
+      begin = d8_first<NT>(p, cut, pref, per, cut.edge(chunk));
+      end = d8_first<NT>(p, cut, pref, per, cut.edge(chunk + 1));
+    }
+  }
 
   if (begin < end) {
     unsigned char* kstage = smem + warp * 2 * Cfg::kTile;
@@ -362,9 +407,8 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
     unsigned char* qstage = smem + NW * 2 * Cfg::kTile + warp * COLS * Cfg::kQRow;
     uint64_t* bar = bars + 2 * warp;     // K, V
     int phase = 0;
-    // up to 32 items of a chunk are in the lanes of `now`, the ones behind them (of the next chunk, at its end) in `next`
-    int n = min(32, end - begin);
-    int next_n = 0, next_begin = 0, next_end = end, next_chunk = chunk;
+    // up to 32 items of the chunk are in the lanes of `now`, the ones behind them in `next`
+    int n = min(32, end - begin), next_n = 0;
     D8Item now = items(begin, n), next = now;
 
     int64_t cur = -1;                    // first row of q of the head the warp is in
@@ -409,14 +453,14 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
           for (int i = 0; i < 4; ++i) acc[mt][0][i] += __shfl_xor_sync(0xffffffffu, acc[mt][0][i], 2);
         if (q4 >= 2) return;             // (the columns of the low parts: their sums are in the other half)
       }
-      float* dst = pieces + (2 * static_cast<int64_t>(chunk) + began) * Cfg::kPiece;
+      float* dst = SHORT ? reinterpret_cast<float*>(kstage) : pieces + (2 * static_cast<int64_t>(chunk) + began) * Cfg::kPiece;
 #pragma unroll
       for (int t = 0; t < CT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int head = 8 * t + 2 * q4 + e;
           if (head >= G) continue;
-          if (began && ends) {
+          if (!SHORT && began && ends) {
             const bool none = l[t][e] == 0.f;
             const float inv = none ? 0.f : __fdividef(1.f, l[t][e]);
 #pragma unroll
@@ -435,25 +479,11 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
         }
     };
 
-    int li = 0, taken = 0;
+    int li = 0;
     for (;;) {
-      const bool tail = begin + n == end;          // these are the chunk's last items
-      if (li == 0 && !tail) {
-        next_begin = begin + n;
-        next_n = min(32, end - next_begin);
-        next = items(next_begin, next_n);
-      }
-      if (tail && cut.nb) {                        // take a chunk, one item ahead of its first load
-        if (li == max(0, n - 2) && lane == 0) taken = atomicAdd(counter, 1);
-        if (li == n - 1) {
-          const uint32_t got = cut.na + __shfl_sync(0xffffffffu, taken, 0);
-          if (got < cut.count()) {
-            next_chunk = static_cast<int>(got);
-            range(got, next_begin, next_end);
-            next_n = min(32, next_end - next_begin);
-            next = items(next_begin, next_n);
-          }
-        }
+      if (li == 0 && begin + n < end) {
+        next_n = min(32, end - begin - n);
+        next = items(begin + n, next_n);
       }
       const bool last = li == n - 1;
       const int b = __shfl_sync(0xffffffffu, now.b, li);
@@ -693,19 +723,68 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
       phase ^= 1;
 
       const bool ends = (info >> 9) & 1;
-      if (ends || (last && tail)) {
-        flush(ends);
-        cur = -1;                        // (a next chunk of the same head is a piece of its own; its q is still in place)
-      }
+      if (ends || begin + li + 1 == end) flush(ends);
+      if (ends) cur = -1;
       if (!last) {
         ++li;
         continue;
       }
       if (next_n == 0) break;
       now = next;
-      li = 0, n = next_n, next_n = 0;
-      begin = next_begin, end = next_end, chunk = next_chunk;
+      begin += n, n = next_n;
+      li = 0, next_n = 0;
     }
+  }
+
+  if constexpr (SHORT) {
+    __shared__ float4 sx[NT];
+    __shared__ float sl[NT], sm[NT];
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();                      // every warp's piece is in its stage
+    const int pieces_n = min(cnt, NW * ranks), all = G * (D / 4);
+    const int quad0 = all * rank / ranks, quads = all * (rank + 1) / ranks - quad0;
+    const int64_t hq0 = static_cast<int64_t>(bs) * p.Hq + hs * G;
+    const uint32_t base = smem_u32(smem);
+    const int S = quads == 0 || quads >= NT ? 1 : min(NT / quads, (pieces_n + 3) / 4);
+    for (int q0 = 0; q0 < quads; q0 += NT) {
+      const int s = S == 1 ? 0 : tid / quads, at = S == 1 ? q0 + tid : tid - s * quads;
+      const bool on = s < S && at < quads;
+      const int quad = quad0 + at, head = quad / (D / 4), d0 = 4 * (quad % (D / 4));
+      float m = -INFINITY, l = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = s; on && c < pieces_n; c += 4 * S) {
+        float pm[4], pl[4];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int y = min(c + i * S, pieces_n - 1);         // piece y: warp y / ranks of CTA y % ranks
+          const uint32_t src = cluster_map(base + (y / ranks) * 2 * Cfg::kTile, y % ranks);
+          pm[i] = cluster_ld_f32(src + (COLS * D + head) * 4);
+          pl[i] = cluster_ld_f32(src + (COLS * D + COLS + head) * 4);
+          v[i] = cluster_ld_f32x4(src + (head * D + d0) * 4);
+        }
+        const float m_old = m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (c + i * S >= pieces_n) pm[i] = -INFINITY, pl[i] = 0.f, v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          m = fmaxf(m, pm[i]);
+        }
+        d8_add<4>(m_old, m, pm, pl, v, l, x);
+      }
+      if (S > 1) {
+        sx[tid] = x, sl[tid] = l, sm[tid] = m;
+        __syncthreads();
+        if (s == 0 && on) d8_join(sx, sl, sm, at, quads, S, m, l, x);
+      }
+      if (s == 0 && on) {
+        d8_store4(p, hq0 + head, d0, x, l);
+        if (d0 == 0) p.lse[hq0 + head] = d8_lse(m, l);
+      }
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();                      // nobody leaves while its pieces are read
   }
 }
 
@@ -715,7 +794,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
 constexpr int D8_MERGE_THREADS = 256;
 template <int D, int MODE>
 __global__ void __launch_bounds__(D8_MERGE_THREADS)
-decode8_merge_kernel(const __grid_constant__ kvskip_decode8_params p, const int warps, const int shared) {
+decode8_merge_kernel(const __grid_constant__ kvskip_decode8_params p, const int warps) {
   using Cfg = D8Cfg<D, MODE>;
   constexpr int COLS = Cfg::kCols, L = D / 4, NT = D8_MERGE_THREADS;
   __shared__ float4 sx[NT];
@@ -750,11 +829,11 @@ decode8_merge_kernel(const __grid_constant__ kvskip_decode8_params p, const int 
     first = span[0], next = span[1];
   } else {
     pdl_wait_prior();
-    const int2* pref = reinterpret_cast<const int2*>(static_cast<const int*>(p.work) + 4);
+    const int2* pref = static_cast<const int2*>(p.work);
     first = pref[u], next = pref[u + 1], total = pref[units];
   }
   const uint32_t count = static_cast<uint32_t>(next.x - first.x) / static_cast<uint32_t>(mul);
-  const D8Chunks cut(total.x, total.y, warps, shared);
+  const D8Chunks cut(total.x, total.y, warps);
   int c0 = 0, c1 = 0;
   if (count) {
     const uint32_t h = p.block_idx ? 0 : bh - b * p.Hkv;
@@ -803,32 +882,12 @@ decode8_merge_kernel(const __grid_constant__ kvskip_decode8_params p, const int 
         if (c + i * S > c1) pm[i] = -INFINITY, pl[i] = 0.f, v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         m = fmaxf(m, pm[i]);
       }
-      const float mu = d8_safe(m), down = ex2(m_old - mu);
-      l *= down;
-      x.x *= down, x.y *= down, x.z *= down, x.w *= down;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = ex2(pm[i] - mu);
-        l += pl[i] * f;
-        x.x += v[i].x * f, x.y += v[i].y * f, x.z += v[i].z * f, x.w += v[i].w * f;
-      }
+      d8_add<8>(m_old, m, pm, pl, v, l, x);
     }
     if (S > 1) {
       sx[tid] = x, sl[tid] = l, sm[tid] = m;
       __syncthreads();
-      if (s == 0 && on) {
-#pragma unroll 8
-        for (int i = 1; i < S; ++i) m = fmaxf(m, sm[i * quads + at]);
-        const float mu = d8_safe(m);
-        l = 0.f, x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int i = 0; i < S; ++i) {
-          const float f = ex2(sm[i * quads + at] - mu);
-          const float4 v = sx[i * quads + at];
-          l += sl[i * quads + at] * f;
-          x.x += v.x * f, x.y += v.y * f, x.z += v.z * f, x.w += v.w * f;
-        }
-      }
+      if (s == 0 && on) d8_join(sx, sl, sm, at, quads, S, m, l, x);
     }
     if (s == 0 && on) {
       d8_store4(p, hq0 + head, d0, x, l);

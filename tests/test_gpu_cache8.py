@@ -120,10 +120,16 @@ def test_decode8_lengths_and_head_layouts(layout, kind, Hkv, G, D, qtype):
     _check(r, ref, D, c["nb"], qtype)
     a = _run(_dev(c), stats=True)
     assert all(torch.equal(r[n], a[n]) for n in ("out", "out_f32", "lse", "blk_max", "blk_sum"))
+    if layout == "paged":     # the same lengths under a far larger bound: another form of the launch
+        c["table"] = torch.cat([c["table"], torch.full((len(LENS), 3000), -1, dtype=torch.int32)], 1)
+        w = _run(_dev(c), stats=True)
+        assert torch.isneginf(w["blk_max"][..., c["nb"]:]).all() and (w["blk_sum"][..., c["nb"]:] == 0).all()
+        _check({**w, **{n: w[n][..., :c["nb"]] for n in ("blk_max", "blk_sum")}}, ref, D, c["nb"], qtype)
     assert K.ext().device_status() == 0
 
 
-@pytest.mark.parametrize("lens", [[1], [64], [65], [0], [0, 0, 5], [4097], [20000], [300] * 70, [130, 0] * 300])
+@pytest.mark.parametrize("lens", [[1], [64], [65], [0], [0, 0, 5], [500], [1024], [2048], [4097], [8192], [20000],
+                                  [300] * 70, [130, 0] * 300])
 def test_decode8_work_split(lens):
     """One short request, one long one over every SM, many of a few blocks, batches larger than a CTA has threads."""
     Hkv = 2 if len(lens) > 4 else 8
@@ -159,9 +165,9 @@ def test_decode8_block_lists(kind, layout, G):
 
 
 @pytest.mark.parametrize("Hkv,T,masked", [(1, 45000 * 64 - 11, False), (2, 23000 * 64, True)])
-def test_decode8_chunks_taken_from_the_counter(Hkv, T, masked):
-    """Enough blocks per warp for the shared part of the work list, in so few heads that every warp takes several chunks
-    of the same one.  The 64-bit sums are formed on the GPU, a stretch of the sequence at a time."""
+def test_decode8_very_long_heads(Hkv, T, masked):
+    """One or two heads over the whole GPU, dozens of blocks per warp.  The 64-bit sums are formed on the GPU, a stretch of
+    the sequence at a time."""
     D, G, B = 64, 4, 1
     gen = torch.Generator(device=DEV).manual_seed(T)
     nb = -(-T // TILE)

@@ -70,7 +70,7 @@ def test_null_blocks_and_sizes(lib):
         assert getattr(lib, f"kvskip_launch_{n}")(None, None) == -1 and b"null" in lib.kvskip_last_error()
     size = lambda **kw: lib.kvskip_decode8_work_bytes(ctypes.byref(_decode_params(**kw)))  # noqa: E731
     assert size(B=0) == 0 and size(nb=0) == 0 and size(block_idx=4096) == 0
-    assert size(Hq=128) > size() > 0 and size(nb=4000) > size()
+    assert size(Hq=128, nb=4000) > size(nb=4000) > size() > 0
 
 
 @pytest.mark.parametrize("change,text", [
