@@ -89,15 +89,15 @@ Decode8Launch decode8_launch(const kvskip_decode8_params& p) {
   Decode8Launch l;
   l.ctas = static_cast<int>(std::min<int64_t>(kvb_host::num_sms(), items));
   l.warps = l.ctas * kvb::D8Cfg<D, MODE>::kWarps;
-  // the short form: as many CTAs per head as give every block a warp, in one wave
+  // the short form: as many CTAs per head as leave four blocks to each of them, in one wave
+  constexpr int kWarps = kvb::D8Cfg<D, MODE, true>::kWarps;
   const int64_t heads = static_cast<int64_t>(p.B) * p.Hkv, longest = p.block_idx ? p.max_blocks : p.nb;
   int c = 1;
-  while (c < 8 && c * kvb::D8Cfg<D, MODE>::kWarps < longest && heads * 2 * c <= kvb_host::num_sms()) c *= 2;
+  while (c < 8 && 4 * c < longest && heads * 2 * c <= kvb_host::num_sms()) c *= 2;
   const bool most = 4 * heads * c >= 3 * kvb_host::num_sms();
   l.cluster = 0;
   // (not for more than 8 query heads: the pieces are four times as large, and joining them so took longer)
-  if (MODE < 2 && heads * c <= kvb_host::num_sms() &&
-      longest <= static_cast<int64_t>(most ? kShortMost : kShortFew) * c * kvb::D8Cfg<D, MODE>::kWarps)
+  if (MODE < 2 && heads * c <= kvb_host::num_sms() && longest <= static_cast<int64_t>(most ? kShortMost : kShortFew) * c * kWarps)
     l.cluster = c;
   return l;
 }
@@ -113,13 +113,14 @@ int64_t decode8_work(const kvskip_decode8_params& p) {
 template <int KIND, int D, int MODE>
 int launch_decode8(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cudaStream_t stream) {
   using Cfg = kvb::D8Cfg<D, MODE>;
+  using Short = kvb::D8Cfg<D, MODE, true>;
   const Decode8Launch l = decode8_launch<D, MODE>(p);
   if constexpr (MODE < 2) {
     if (l.cluster) {
       auto kernel = kvb::decode8_kernel<KIND, D, MODE, true>;
-      if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmem)) return rc;
-      KVB_CUDA(launch_cluster(kernel, dim3(static_cast<unsigned>(p.B) * p.Hkv * l.cluster), Cfg::kThreads,
-                              static_cast<unsigned>(l.cluster), Cfg::kSmem, stream, p, maps));
+      if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Short::kSmem)) return rc;
+      KVB_CUDA(launch_cluster(kernel, dim3(static_cast<unsigned>(p.B) * p.Hkv * l.cluster), Short::kThreads,
+                              static_cast<unsigned>(l.cluster), Short::kSmem, stream, p, maps));
       return KVSKIP_OK;
     }
   }

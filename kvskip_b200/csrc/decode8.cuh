@@ -35,12 +35,14 @@ struct D8Maps {
 };
 
 // MODE 0: G <= 4, one column tile with high and low parts; 1: G <= 8, one tile; 2: G <= 16, two tiles.
-template <int D, int MODE>
+// Warps: as many as keep the memory busy and no more, since a deeper queue in front of it is shared out unevenly between the
+// SMs (batch 16 / 64k: 320 us with 7, 327 with 8, 344 with 10, 364 with 12; batch 1 / 64k: 29.7, 29.5, 34.1, 40.4).
+template <int D, int MODE, bool SHORT = false>
 struct D8Cfg {
   static constexpr int kCols = MODE == 0 ? 4 : MODE == 1 ? 8 : 16;   // query heads there is room for
   static constexpr int kTiles = MODE == 2 ? 2 : 1;
   static constexpr int kParts = MODE == 0 ? 1 : 2;                   // MMA instructions per P fragment
-  static constexpr int kWarps = MODE == 2 || D == 128 ? 8 : 12;
+  static constexpr int kWarps = D == 64 && MODE < 2 ? 12 : MODE == 0 && !SHORT ? 7 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kTile = TILE * D;                             // bytes of a K or V tile
   static constexpr int kQRow = 2 * D + 16;                           // bytes of a q row in shared memory, conflict-free
@@ -293,9 +295,9 @@ __device__ __forceinline__ float4 cluster_ld_f32x4(const uint32_t addr) {
 // head's blocks evenly; the pieces stay in shared memory and the CTAs of the cluster join a share of the output each,
 // reading the others' through distributed shared memory.  No list, no second launch.
 template <int KIND, int D, int MODE, bool SHORT>
-__global__ void __launch_bounds__(D8Cfg<D, MODE>::kThreads, 1)
+__global__ void __launch_bounds__(D8Cfg<D, MODE, SHORT>::kThreads, 1)
 decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_constant__ D8Maps maps) {
-  using Cfg = D8Cfg<D, MODE>;
+  using Cfg = D8Cfg<D, MODE, SHORT>;
   constexpr int NW = Cfg::kWarps, NT = Cfg::kThreads, KS = D / 16;
   constexpr int CT = Cfg::kTiles, PT = Cfg::kParts, COLS = Cfg::kCols;
 
