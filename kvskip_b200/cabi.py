@@ -172,6 +172,46 @@ class CAbi:
         self._keep = (pacc, pml)   # scratch must outlive the asynchronous launch
         return [out, lse, bmax, bsum, o32, pbuf]
 
+    @staticmethod
+    def _cache8(p, k, v, k_scale, v_scale):
+        p.k, p.v, p.k_scale, p.v_scale = _ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale)
+        p.k_sb, p.k_sh, p.k_st = k.stride()[:3]
+        p.v_sb, p.v_sh, p.v_st = v.stride()[:3]
+        p.ks_sb, p.ks_sh, p.ks_st = (*k_scale.stride(), 0)[:3]
+        p.vs_sb, p.vs_sh, p.vs_st = (*v_scale.stride(), 0)[:3]
+        p.kind = int(k.dtype == torch.int8)
+        p.Hkv, p.D = k.shape[1], k.shape[3]
+
+    def decode8(self, q, k, v, k_scale, v_scale, scale, lens=None, page_table=None):
+        """kvskip_launch_decode8 with every buffer from the caller's side; returns [out, lse]."""
+        p = Decode8Params()
+        self._cache8(p, k, v, k_scale, v_scale)
+        B, Hq, D = q.shape
+        p.q, p.q_sb, p.q_sh, p.q_f16 = _ptr(q), q.stride(0), q.stride(1), int(q.dtype == torch.float16)
+        p.B, p.Hq, p.T = B, Hq, k.shape[2]
+        if page_table is not None:
+            p.page_table, p.max_pages, p.num_pages = _ptr(page_table), page_table.shape[1], k.shape[0]
+            p.T = page_table.shape[1] * TILE
+        p.nb, p.lens, p.scale_log2 = math.ceil(p.T / TILE), _ptr(lens), scale * 1.4426950408889634
+        out, lse = torch.empty_like(q), torch.empty(B, Hq, dtype=torch.float32, device=q.device)
+        size = getattr(self.lib, f"{self.prefix}_decode8_work_bytes")
+        size.restype = _i64
+        work = torch.empty(size(C.byref(p)), dtype=torch.uint8, device=q.device)
+        p.out, p.lse, p.work = _ptr(out), _ptr(lse), _ptr(work)
+        self._call("decode8", C.byref(p), _stream())
+        self._keep = work          # scratch must outlive the asynchronous launch
+        return [out, lse]
+
+    def write8(self, k_new, v_new, slots, k, v, k_scale, v_scale):
+        """kvskip_launch_write8 into a page pool, k_new and v_new [N,Hkv,D]."""
+        p = Write8Params()
+        self._cache8(p, k, v, k_scale, v_scale)
+        p.k_new, p.v_new, p.slots = _ptr(k_new), _ptr(v_new), _ptr(slots)
+        p.kn_si, p.kn_sh, p.vn_si, p.vn_sh = *k_new.stride()[:2], *v_new.stride()[:2]
+        p.n = p.inner = slots.numel()
+        p.x_f16, p.blocks, p.tokens, p.num_blocks = int(k_new.dtype == torch.float16), 1, TILE, k.shape[0]
+        self._call("write8", C.byref(p), _stream())
+
     def vskip1(self, q, k, v, scale, tau, local=2, num_splits=1, want_f32=False, count=False, lse_prev=None):
         B, Hq, D = q.shape
         Hkv, T = k.shape[1], k.shape[2]

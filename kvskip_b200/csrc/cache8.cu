@@ -234,6 +234,7 @@ int kvskip_launch_decode8(const kvskip_decode8_params* p, void* stream) {
   if (p->kind != KVSKIP_KIND_E4M3 && p->kind != KVSKIP_KIND_INT8) return fail(KVSKIP_E_ARG, "decode8: kind 0 (e4m3) or 1 (int8)");
   if (p->B < 1 || p->Hkv < 1 || p->T < 1 || p->Hq < 1 || p->Hq % p->Hkv) return fail(KVSKIP_E_ARG, "decode8: bad B / Hq / Hkv / T");
   if (p->Hq / p->Hkv > 16) return fail(KVSKIP_E_ARG, "decode8: at most 16 query heads per KV head");
+  if (p->Hkv > 1 << 20) return fail(KVSKIP_E_LIMIT, "decode8: more than 2^20 KV heads");
   if (!p->q || !p->k || !p->v || !p->k_scale || !p->v_scale || !p->out || !p->lse || !p->work)
     return fail(KVSKIP_E_ARG, "decode8: q, k, v, k_scale, v_scale, out, lse and work are required");
   if (p->nb != (p->T - 1) / KVSKIP_TILE + 1) return fail(KVSKIP_E_ARG, "decode8: nb must be ceil(T / 64)");

@@ -732,6 +732,8 @@ void same_device(const at::Tensor& a, std::initializer_list<const at::Tensor*> o
 int check_cache8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks, const at::Tensor& vs, bool paged) {
   const int kind = kind_of(k, "k");
   TORCH_CHECK(kind_of(v, "v") == kind && v.sizes() == k.sizes(), "k and v must share type and shape");
+  TORCH_CHECK(k.numel() > 0 && k.size(0) < (1LL << 31) && k.size(1) < (1LL << 20) && k.size(2) < (1LL << 31) - KVSKIP_TILE,
+              "an empty cache, or one with more than 2^31 pages or tokens");
   TORCH_CHECK(ks.is_cuda() && vs.is_cuda() && ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat,
               "k_scale, v_scale: CUDA fp32");
   if (paged) {

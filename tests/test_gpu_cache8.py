@@ -256,6 +256,39 @@ def test_decode8_nan_stays_in_its_row():
     assert torch.equal(r["out_f32"][0, G:], clean["out_f32"][0, G:]) and torch.equal(r["out_f32"][1], clean["out_f32"][1])
 
 
+@pytest.mark.parametrize("G,bound", [(4, 6), (8, 6), (4, 4000), (16, 6)])
+def test_decode8_lists_without_a_token_and_negative_scale(G, bound):
+    """A list of blocks behind the length reads nothing; the sign of the softmax scale is free."""
+    lens, Hkv, D = [70, 300], 2, 128
+    c = _case(lens, Hkv, G, D, "e4m3", torch.bfloat16, "paged", seed=G + bound, T=bound * TILE)
+    c["scale"] = -0.05
+    nb = c["nb"]
+    keep = torch.zeros(2, Hkv, nb, dtype=torch.bool)
+    keep[0, 0, 4:6] = True                                         # behind the length: nothing
+    keep[0, 1, 0] = keep[0, 1, 5] = True
+    keep[1] = True
+    lists = {(b, h): torch.nonzero(keep[b, h])[:, 0].tolist() for b in range(2) for h in range(Hkv)}
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], lens, c["table"], lists)
+    r = _run(_dev(c), plan=K.make_plan(keep.to(DEV)), stats=True)
+    _check(r, ref, D, nb, torch.bfloat16)
+    assert (r["out_f32"][0, :G] == 0).all() and torch.isneginf(r["lse"][0, :G]).all()
+
+
+def test_c_entry_points_give_the_same_bits():
+    from kvskip_b200.cabi import CAbi
+    lib = CAbi()
+    c = _dev(_case([200, 0, 65], 2, 4, 128, "int8", torch.float16, "paged", seed=3))
+    out, lse = lib.decode8(c["q"], c["k"], c["v"], c["ks"], c["vs"], c["scale"], c["lens"], c["table"])
+    r = _run(c)
+    assert torch.equal(out, r["out"]) and torch.equal(lse, r["lse"])
+    x = torch.randn(2, 70, 2, 128, device=DEV).to(torch.float16)
+    slots = torch.arange(64, 134, device=DEV)
+    a, b = ([t.clone() for t in (c["k"], c["v"], c["ks"], c["vs"])] for _ in range(2))
+    lib.write8(x[0], x[1], slots, *a)
+    K.write8(x[0], x[1], slots, *b)
+    assert all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(a, b))
+
+
 def test_decode8_pages_outside_the_pool_read_as_zeros():
     lens = [200, 70]
     c = _case(lens, 2, 4, 128, "e4m3", torch.bfloat16, "paged", seed=6)
@@ -457,6 +490,47 @@ def test_write8_skips_and_reports_bad_slots():
     K.write8(x[:2].to(DEV), x[:2].to(DEV), torch.tensor([99, 100], device=DEV), k, k.clone(), s, s.clone())
     assert K.ext().device_status() == 0x302
     assert (k[:, :, :99] == 0).all() and (k[:, :, 99] != 0).any()
+
+
+def test_write8_inputs_without_a_tensor_map():
+    """One key for every head (a stride of 0), and a run that goes on in the next row of a padded list."""
+    Hkv, D, gen = 4, 128, torch.Generator().manual_seed(8)
+    codes, scales = _pool(5, Hkv, D, "e4m3", gen)
+    x = torch.randn(80, 1, D, generator=gen).to(torch.bfloat16)
+    slots = torch.cat([torch.arange(64, 128), torch.arange(128 + 40, 128 + 56)])
+    _write_both(x.expand(80, Hkv, D), slots, codes, scales, "e4m3", k4=lambda t: t[:, :1].contiguous().expand(80, Hkv, D))
+    x = torch.randn(80, Hkv, D, generator=gen).to(torch.bfloat16)
+    rows = lambda t: t.view(4, 20, Hkv, D).transpose(1, 2)                      # noqa: E731
+    want_c, want_s = codes.view(torch.uint8).numpy().copy(), scales.numpy().copy()
+    R.write_ref(x.float().numpy(), slots.tolist(), want_c, want_s, "e4m3")
+    k, ks = codes.to(DEV), scales.to(DEV)
+    v, vs = k.clone(), ks.clone()
+    K.write8(rows(x.to(DEV)), rows(x.to(DEV)), slots.view(4, 20).to(DEV), k, v, ks, vs)
+    assert _same_codes(k.view(torch.uint8).cpu().numpy(), want_c, "e4m3") and np.array_equal(ks.cpu().numpy(), want_s)
+    assert torch.equal(k.view(torch.uint8), v.view(torch.uint8)) and torch.equal(ks, vs)
+
+
+@pytest.mark.parametrize("n", [300, 2500, 9000])
+def test_write8_many_tokens_of_many_requests(n):
+    """Single tokens and short runs in numbers that take every chunk size of the slot list, V unlike K."""
+    Hkv, D, gen = 8, 64, torch.Generator().manual_seed(n)
+    runs, left = [], n
+    while left:
+        m = min(left, int(torch.randint(1, 4, (1,), generator=gen)) if len(runs) % 7 else 1 + len(runs) % 64)
+        runs.append(m)
+        left -= m
+    codes, scales = _pool(len(runs), Hkv, D, "int8", gen)
+    order = torch.randperm(len(runs), generator=gen).tolist()
+    start = [int(torch.randint(0, 65 - m, (1,), generator=gen)) for m in runs]
+    slots = torch.tensor([order[i] * TILE + start[i] + j for i, m in enumerate(runs) for j in range(m)])
+    x, y = (torch.randn(n, Hkv, D, generator=gen).to(torch.bfloat16) for _ in range(2))
+    k, ks = codes.to(DEV), scales.to(DEV)
+    v, vs = k.clone(), ks.clone()
+    K.write8(x.to(DEV), y.to(DEV), slots.to(DEV), k, v, ks, vs)
+    for t, c, s in ((x, k, ks), (y, v, vs)):
+        want_c, want_s = codes.view(torch.uint8).numpy().copy(), scales.numpy().copy()
+        R.write_ref(t.float().numpy(), slots.tolist(), want_c, want_s, "int8")
+        assert np.array_equal(s.cpu().numpy(), want_s) and np.array_equal(c.view(torch.uint8).cpu().numpy(), want_c)
 
 
 # ------------------------------------------------------------------------------------------ pages

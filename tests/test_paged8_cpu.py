@@ -54,7 +54,7 @@ def _decode_params(**kw):
 
 @pytest.mark.parametrize("change,text", [
     (dict(D=96), b"head dim"), (dict(kind=2), b"kind"), (dict(B=0), b"bad B"), (dict(Hq=30), b"bad B"),
-    (dict(Hq=17 * 8), b"at most 16"), (dict(T=0, nb=0), b"bad B"), (dict(q=0), b"required"), (dict(work=0), b"required"),
+    (dict(Hq=17 * 8), b"at most 16"), (dict(Hkv=1 << 21, Hq=1 << 21), b"2^20"), (dict(T=0, nb=0), b"bad B"), (dict(q=0), b"required"), (dict(work=0), b"required"),
     (dict(nb=3), b"nb must be"), (dict(block_idx=4096), b"go together"), (dict(blk_max=4096), b"go together"),
     (dict(page_table=4096, max_pages=1, num_pages=9), b"page table"), (dict(page_table=4096, max_pages=2), b"page table"),
     (dict(page_table=4096, max_pages=2, num_pages=9, lens=0), b"needs lens"), (dict(q=4100), b"8-byte"),
