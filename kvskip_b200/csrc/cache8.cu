@@ -90,7 +90,7 @@ Decode8Launch decode8_launch(const kvskip_decode8_params& p) {
   l.ctas = static_cast<int>(std::min<int64_t>(kvb_host::num_sms(), items));
   l.warps = l.ctas * kvb::D8Cfg<D, MODE>::kWarps;
   // the short form: as many CTAs per head as leave four blocks to each of them, in one wave
-  constexpr int kWarps = kvb::D8Cfg<D, MODE, true>::kWarps;
+  constexpr int kWarps = kvb::D8Cfg<D, MODE>::kWarps;
   const int64_t heads = static_cast<int64_t>(p.B) * p.Hkv, longest = p.block_idx ? p.max_blocks : p.nb;
   int c = 1;
   while (c < 8 && 4 * c < longest && heads * 2 * c <= kvb_host::num_sms()) c *= 2;
@@ -113,14 +113,13 @@ int64_t decode8_work(const kvskip_decode8_params& p) {
 template <int KIND, int D, int MODE>
 int launch_decode8(const kvskip_decode8_params& p, const kvb::D8Maps& maps, cudaStream_t stream) {
   using Cfg = kvb::D8Cfg<D, MODE>;
-  using Short = kvb::D8Cfg<D, MODE, true>;
   const Decode8Launch l = decode8_launch<D, MODE>(p);
   if constexpr (MODE < 2) {
     if (l.cluster) {
       auto kernel = kvb::decode8_kernel<KIND, D, MODE, true>;
-      if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Short::kSmem)) return rc;
-      KVB_CUDA(launch_cluster(kernel, dim3(static_cast<unsigned>(p.B) * p.Hkv * l.cluster), Short::kThreads,
-                              static_cast<unsigned>(l.cluster), Short::kSmem, stream, p, maps));
+      if (int rc = kvb_host::ensure_smem(reinterpret_cast<const void*>(kernel), Cfg::kSmem)) return rc;
+      KVB_CUDA(launch_cluster(kernel, dim3(static_cast<unsigned>(p.B) * p.Hkv * l.cluster), Cfg::kThreads,
+                              static_cast<unsigned>(l.cluster), Cfg::kSmem, stream, p, maps));
       return KVSKIP_OK;
     }
   }
@@ -191,7 +190,7 @@ int by_type(const kvskip_write8_params& p, cudaStream_t s) {
 
 // CTAs for `n` table or slot entries (200k slots, B200: 7.7 us with 4096 of them per CTA, 6.2 with 2048, 5.5 with 1024)
 int pages_grid(int64_t n) {
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kvb_host::num_sms(), n / 4096)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kvb_host::num_sms(), n / 1024)));
 }
 
 int check_pages(const kvskip_pages_params* p, const char* who) {

@@ -36,13 +36,14 @@ struct D8Maps {
 
 // MODE 0: G <= 4, one column tile with high and low parts; 1: G <= 8, one tile; 2: G <= 16, two tiles.
 // Warps: as many as keep the memory busy and no more, since a deeper queue in front of it is shared out unevenly between the
-// SMs (batch 16 / 64k: 320 us with 7, 327 with 8, 344 with 10, 364 with 12; batch 1 / 64k: 29.7, 29.5, 34.1, 40.4).
-template <int D, int MODE, bool SHORT = false>
+// SMs (batch 16 / 64k in a loop of 0.3 s, under the power cap: 346 us with 7, 330 with 8, 372 with 10, 369 with 12; batch 1 /
+// 64k: 29.3, 29.5, 34.8, 40.5).
+template <int D, int MODE>
 struct D8Cfg {
   static constexpr int kCols = MODE == 0 ? 4 : MODE == 1 ? 8 : 16;   // query heads there is room for
   static constexpr int kTiles = MODE == 2 ? 2 : 1;
   static constexpr int kParts = MODE == 0 ? 1 : 2;                   // MMA instructions per P fragment
-  static constexpr int kWarps = D == 64 && MODE < 2 ? 12 : MODE == 0 && !SHORT ? 7 : 8;
+  static constexpr int kWarps = D == 64 && MODE < 2 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kTile = TILE * D;                             // bytes of a K or V tile
   static constexpr int kQRow = 2 * D + 16;                           // bytes of a q row in shared memory, conflict-free
@@ -295,9 +296,9 @@ __device__ __forceinline__ float4 cluster_ld_f32x4(const uint32_t addr) {
 // head's blocks evenly; the pieces stay in shared memory and the CTAs of the cluster join a share of the output each,
 // reading the others' through distributed shared memory.  No list, no second launch.
 template <int KIND, int D, int MODE, bool SHORT>
-__global__ void __launch_bounds__(D8Cfg<D, MODE, SHORT>::kThreads, 1)
+__global__ void __launch_bounds__(D8Cfg<D, MODE>::kThreads, 1)
 decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_constant__ D8Maps maps) {
-  using Cfg = D8Cfg<D, MODE, SHORT>;
+  using Cfg = D8Cfg<D, MODE>;
   constexpr int NW = Cfg::kWarps, NT = Cfg::kThreads, KS = D / 16;
   constexpr int CT = Cfg::kTiles, PT = Cfg::kParts, COLS = Cfg::kCols;
 
@@ -414,26 +415,31 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
     D8Item now = items(begin, n), next = now;
 
     int64_t cur = -1;                    // first row of q of the head the warp is in
-    auto load = [&](const D8Item& from, const int i, const bool is_v) {
-      const int h = __shfl_sync(0xffffffffu, from.info, i) >> 10;
+    int at_h = 0, at_t = 0, at_n = 0;    // head, row and page (or sequence) of the block that is loaded next
+    auto load_k = [&](const D8Item& from, const int i) {
+      at_h = __shfl_sync(0xffffffffu, from.info, i) >> 10;
       const int blk = __shfl_sync(0xffffffffu, from.blk, i);
-      const int page = __shfl_sync(0xffffffffu, from.page, i);
+      at_n = __shfl_sync(0xffffffffu, from.page, i);
+      at_t = p.page_table ? 0 : blk * TILE;
       if (lane == 0) {
-        mbar_expect_tx(&bar[is_v], Cfg::kTile);
-        tma_load_4d(is_v ? vstage : kstage, is_v ? &maps.v : &maps.k, &bar[is_v], 0, p.page_table ? 0 : blk * TILE,
-                    h, page);
+        mbar_expect_tx(&bar[0], Cfg::kTile);
+        tma_load_4d(kstage, &maps.k, &bar[0], 0, at_t, at_h, at_n);
       }
-      if (!is_v) {                       // another head: its rows of q come along
-        const int b = __shfl_sync(0xffffffffu, from.b, i);
-        if (static_cast<int64_t>(b) * p.Hq + h * G != cur) {
-          const uint16_t* src = p.q + b * p.q_sb + static_cast<int64_t>(h) * G * p.q_sh;
-          for (int o = lane; o < G * (D / 4); o += 32)
-            cp_async8(smem_u32(qstage + o / (D / 4) * Cfg::kQRow + o % (D / 4) * 8), src + o / (D / 4) * p.q_sh + o % (D / 4) * 4);
-        }
+      const int b = __shfl_sync(0xffffffffu, from.b, i);
+      if (static_cast<int64_t>(b) * p.Hq + at_h * G != cur) {        // another head: its rows of q come along
+        const uint16_t* src = p.q + b * p.q_sb + static_cast<int64_t>(at_h) * G * p.q_sh;
+        for (int o = lane; o < G * (D / 4); o += 32)
+          cp_async8(smem_u32(qstage + o / (D / 4) * Cfg::kQRow + o % (D / 4) * 8), src + o / (D / 4) * p.q_sh + o % (D / 4) * 4);
       }
     };
-    load(now, 0, false);
-    load(now, 0, true);
+    auto load_v = [&]() {                // of the block whose K was loaded last
+      if (lane == 0) {
+        mbar_expect_tx(&bar[1], Cfg::kTile);
+        tma_load_4d(vstage, &maps.v, &bar[1], 0, at_t, at_h, at_n);
+      }
+    };
+    load_k(now, 0);
+    load_v();
 
     uint32_t bq[CT][KS][2];
     float cm[CT][2];                       // softmax scale / row scale of q of this thread's two columns
@@ -596,8 +602,8 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
         }
       }
       __syncwarp();
-      if (!last) load(now, li + 1, false);
-      else if (next_n > 0) load(next, 0, false);
+      if (!last) load_k(now, li + 1);
+      else if (next_n > 0) load_k(next, 0);
 
       // ---- softmax relative to the block's own maximum, joined with the running one
       uint32_t pb[CT][4][PT][2];
@@ -673,18 +679,22 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
       }
 
       if (!mbar_wait(&bar[1], phase, 0x620u + warp)) break;
-      // V rows behind the length: their weights are zero, but zero times a NaN code is not (int8 has none)
-      uint32_t vmask[8];
-      if constexpr (KIND == KVSKIP_KIND_E4M3) {
-#pragma unroll
-        for (int m = 0; m < 8; ++m) {
-          const int t = m * 8 + 2 * q4;          // a register of the fragment holds two codes of tokens t and t + 1 each
-          vmask[m] = t + 1 < tok ? 0xffffffffu : t < tok ? 0xffffu : 0u;
-        }
+      if (KIND == KVSKIP_KIND_E4M3 && tok < TILE) {
+        // V rows behind the length: their weights are zero, but zero times a NaN code is not (int8 has none)
+        for (int o = tok * D + lane * 16; o < TILE * D; o += 512) *reinterpret_cast<uint4*>(vstage + o) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();          // ordered before the next load into this stage
+        __syncwarp();
       }
       // ---- O^T = alpha O^T + beta vs V^T P^T: row g of a tile is channel 2 g, row g + 8 channel 2 g + 1
       // (two adjacent codes of a token travel as one 16-bit unit through the transposing ldmatrix)
-      rescale = __any_sync(0xffffffffu, rescale);
+      if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+          for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[mt][t][e] *= alpha[t][e & 1];
+      }
 #pragma unroll
       for (int mt = 0; mt < KS; ++mt) {
         float tmp[CT][4];
@@ -696,10 +706,6 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
         for (int th = 0; th < 2; ++th) {
           uint32_t r[4];
           ldsm_x4_t(r, at(vt, th * 32 + lmat * 8 + lrow, mt));
-          if constexpr (KIND == KVSKIP_KIND_E4M3) {
-#pragma unroll
-            for (int m = 0; m < 4; ++m) r[m] &= vmask[th * 4 + m];
-          }
 #pragma unroll
           for (int kk = 0; kk < 2; ++kk) {
             uint32_t a[4];
@@ -714,14 +720,10 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
 #pragma unroll
         for (int t = 0; t < CT; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (rescale) acc[mt][t][e] *= alpha[t][e & 1];
-            acc[mt][t][e] += beta[t][e & 1] * tmp[t][e];
-          }
+          for (int e = 0; e < 4; ++e) acc[mt][t][e] += beta[t][e & 1] * tmp[t][e];
       }
       __syncwarp();
-      if (!last) load(now, li + 1, true);
-      else if (next_n > 0) load(next, 0, true);
+      if (!last || next_n > 0) load_v();
       phase ^= 1;
 
       const bool ends = (info >> 9) & 1;
