@@ -753,28 +753,33 @@ int check_cache8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& ks,
 at::Tensor new_cuda(at::IntArrayRef shape, at::ScalarType type, const at::Device& device) {
   return at::detail::empty_cuda(shape, type, device, c10::nullopt);
 }
-// Several tensors in one allocation (each 256-byte aligned): one trip to the allocator instead of one per tensor.
+// Up to six tensors of at most two dims in one allocation (each 256-byte aligned): one trip to the allocator.
 struct NewTogether {
-  std::vector<std::pair<at::Tensor*, std::pair<c10::SmallVector<int64_t, 2>, at::ScalarType>>> parts;
+  struct Part {
+    at::Tensor* t;
+    int64_t shape[2];
+    int dims;
+    at::ScalarType type;
+    int64_t bytes;
+  } parts[6];
+  int n = 0;
+  int64_t total = 0;
   void add(at::Tensor& t, at::IntArrayRef shape, at::ScalarType type) {
-    parts.push_back({&t, {c10::SmallVector<int64_t, 2>(shape.begin(), shape.end()), type}});
+    Part& p = parts[n++];
+    p = {&t, {shape[0], shape.size() > 1 ? shape[1] : 1}, static_cast<int>(shape.size()), type, 0};
+    p.bytes = (p.shape[0] * p.shape[1] * static_cast<int64_t>(c10::elementSize(type)) + 255) / 256 * 256;
+    total += p.bytes;
   }
   void make(const at::Device& device) {
-    const auto bytes = [](const c10::SmallVector<int64_t, 2>& shape, const at::ScalarType type) {
-      int64_t n = static_cast<int64_t>(c10::elementSize(type));
-      for (const int64_t d : shape) n *= d;
-      return (n + 255) / 256 * 256;
-    };
-    int64_t total = 0;
-    for (const auto& p : parts) total += bytes(p.second.first, p.second.second);
+    if (n == 0) return;
     const at::Tensor all = new_cuda({total}, at::kByte, device);
     int64_t at_byte = 0;
-    for (const auto& p : parts) {
-      const at::ScalarType type = p.second.second;
-      *p.first = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
-      p.first->unsafeGetTensorImpl()->set_storage_offset(at_byte / static_cast<int64_t>(c10::elementSize(type)));
-      p.first->unsafeGetTensorImpl()->set_sizes_contiguous(p.second.first);
-      at_byte += bytes(p.second.first, type);
+    for (int i = 0; i < n; ++i) {
+      const Part& p = parts[i];
+      *p.t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(p.type));
+      p.t->unsafeGetTensorImpl()->set_storage_offset(at_byte / static_cast<int64_t>(c10::elementSize(p.type)));
+      p.t->unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(p.shape, p.dims));
+      at_byte += p.bytes;
     }
   }
 };
@@ -928,9 +933,9 @@ void fill_pages(kvskip_pages_params& p, const at::Tensor& lens, const at::Tensor
   TORCH_CHECK(free_pages.dim() == 1 && free_pages.size(0) >= 1 && n_free.numel() == 1, "free_pages: [pages], n_free: one element");
   same_device(lens, {&page_table, &free_pages, &n_free});
   if (lens_out.has_value()) lo = *lens_out;
-  else fresh.add(lo, lens.sizes(), at::kInt);
+  else fresh.add(lo, lens.sizes(), at::kInt);        // (checked above: one dim)
   if (n_free_out.has_value()) fo = *n_free_out;
-  else fresh.add(fo, n_free.sizes(), at::kInt);
+  else fresh.add(fo, {1}, at::kInt);
   fresh.make(lens.device());
   p.lens_out = const_cast<int32_t*>(i32(lo, "lens_out"));
   p.n_free_out = const_cast<int32_t*>(i32(fo, "n_free_out"));
