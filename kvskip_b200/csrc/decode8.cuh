@@ -12,8 +12,8 @@
 //
 // Work split: the (sequence, head, block) items of the whole launch are one list, ordered by sequence,
 // head and block, cut evenly into one chunk per warp.  So requests of any mixture of lengths keep every SM busy to the end
-// without the host knowing a length.  A warp keeps the running maximum, sum
-// and output of the head it is in and has its own stage (a K and a V tile with an mbarrier each, refilled as soon as
+// without the host knowing a length.  A warp keeps the running maximum, sum and output of the head it is in and has its own
+// stage (a K and a V tile with an mbarrier each, refilled as soon as
 // its products are done): no barrier between warps anywhere.  A head that a chunk holds from its first to its last
 // block is written out by the warp; other pieces (at most two per chunk) go to `work` and are joined, in item order,
 // by decode8_merge_kernel.  Nothing is added in an order that depends on timing.  (Chunks taken from a counter, so that SMs
@@ -347,28 +347,28 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
   const int per = (units + NT - 1) / NT;
   int2 mine = make_int2(0, 0), total = make_int2(0, 0);
   if constexpr (!SHORT) {
-  for (int u = tid * per; u < min(units, (tid + 1) * per); ++u) {
-    const int n = d8_count(p, u);
-    mine.x += n * mul, mine.y += n ? mul : 0;
-  }
-  int2 incl = mine;
+    for (int u = tid * per; u < min(units, (tid + 1) * per); ++u) {
+      const int n = d8_count(p, u);
+      mine.x += n * mul, mine.y += n ? mul : 0;
+    }
+    int2 incl = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
-    if (lane >= o) incl.x += x, incl.y += y;
-  }
-  if (lane == 31) wsum[warp] = incl;
-  __syncthreads();
-  int2 before = make_int2(0, 0);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+      if (lane >= o) incl.x += x, incl.y += y;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    int2 before = make_int2(0, 0);
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const int2 t = wsum[w];
-    if (w < warp) before.x += t.x, before.y += t.y;
-    total.x += t.x, total.y += t.y;
-  }
-  pref[tid] = make_int2(before.x + incl.x - mine.x, before.y + incl.y - mine.y);
-  if (tid == 0) pref[NT] = total;
-  __syncthreads();
+    for (int w = 0; w < NW; ++w) {
+      const int2 t = wsum[w];
+      if (w < warp) before.x += t.x, before.y += t.y;
+      total.x += t.x, total.y += t.y;
+    }
+    pref[tid] = make_int2(before.x + incl.x - mine.x, before.y + incl.y - mine.y);
+    if (tid == 0) pref[NT] = total;
+    __syncthreads();
   }
 
   float* pieces = static_cast<float*>(p.work) + d8_piece_base(units);

@@ -375,11 +375,26 @@ def write8(k_new, v_new, slots, k, v, k_scale, v_scale) -> None:
     them.  The scale of a block is the smallest power of two that covers its values so far; when a token
     makes it grow, the codes already there are rounded to the new scale.  A token in row 0 starts its block
     afresh, whatever page and scale held before.  Infinities saturate; a NaN stays one in e4m3 and is 0 in int8.
-    A slot outside the cache is skipped and sets the status word (`check_status`)."""
+    A slot outside the cache is skipped and sets the status word (`check_status`).  Two runs of one block in a call race
+    for it unless they are neighbours (then the second is skipped, with the status word set); KVSKIP_CHECK_STATUS=1
+    refuses them."""
     e = _EXT or ext()
+    checked = e.check_wanted()
+    if checked:
+        _check_runs(slots)
     e.write8(k_new, v_new, slots, k, v, k_scale, v_scale)
-    if e.check_wanted():
+    if checked:
         check_status("write8")
+
+
+def _check_runs(slots) -> None:
+    """Raises ValueError if a block's tokens are not one run of the slot list (reads the list back)."""
+    s = slots.reshape(-1)
+    before = torch.cat([s.new_full((1,), -1), s[:-1]])
+    first = (s >= 0) & ~((before >= 0) & (s == before + 1) & (s % TILE != 0))
+    blocks = s[first] // TILE
+    if blocks.unique().numel() != blocks.numel():
+        raise ValueError("write8: the tokens of a block must stand next to each other in `slots`, with ascending rows")
 
 
 def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | None = None, per_row: int | None = None,

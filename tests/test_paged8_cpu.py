@@ -134,3 +134,12 @@ def test_front_end_argument_errors():
         PagedKV8(1, 1, 1, 96, 64, "cpu")
     with pytest.raises(ValueError, match="at least 1"):
         PagedKV8(0, 1, 1, 64, 64, "cpu")
+
+
+def test_debug_check_of_the_slot_list():
+    K._check_runs(torch.tensor([5, 6, 7, -1, 64, 65, 128, -1, -1, 200]))
+    K._check_runs(torch.tensor([[62, 63], [64, 65]]))
+    K._check_runs(torch.tensor([], dtype=torch.int64))
+    for bad in ([5, 5], [5, 7], [5, 64, 6], [7, -1, 8], [6, 5]):
+        with pytest.raises(ValueError, match="next to each other"):
+            K._check_runs(torch.tensor(bad))
