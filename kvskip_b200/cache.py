@@ -204,8 +204,8 @@ class PagedKV8:
         self._ones = torch.ones(B, dtype=torch.int32, device=device)
 
     def extend(self, new: torch.Tensor | None = None, *, n_tokens: int | None = None, per_row: int | None = None):
-        """Room for new[b] (int32 [B], default one) more tokens of every request; returns their slots (see
-        `kvskip.extend_pages`), `granted` and `positions` are kept on the object."""
+        """Room for new[b] (int32 [B], default one in every row, rows of length 0 too) more tokens of every request;
+        returns their slots (see `kvskip.extend_pages`), `granted` and `positions` are kept on the object."""
         if new is None:
             new = self._ones
         if n_tokens is None and per_row is None:

@@ -37,7 +37,8 @@ struct D8Maps {
 // MODE 0: G <= 4, one column tile with high and low parts; 1: G <= 8, one tile; 2: G <= 16, two tiles.
 // Warps: as many as keep the memory busy and no more, since a deeper queue in front of it is shared out unevenly between the
 // SMs (batch 16 / 64k in a loop of 0.3 s, under the power cap: 346 us with 7, 330 with 8, 372 with 10, 369 with 12; batch 1 /
-// 64k: 29.3, 29.5, 34.8, 40.5).
+// 64k: 29.3, 29.5, 34.8, 40.5).  Fewer warps with two stages each are behind too, with one tile of columns at D 128 (6, 5 and 4
+// of them: 349, 375, 388 us for batch 16 / 64k; 34.3, 32.5, 31.9 for batch 1): a warp's own instructions become the bound.
 template <int D, int MODE>
 struct D8Cfg {
   static constexpr int kCols = MODE == 0 ? 4 : MODE == 1 ? 8 : 16;   // query heads there is room for

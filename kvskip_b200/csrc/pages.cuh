@@ -11,7 +11,8 @@
 namespace kvb {
 
 constexpr int PG_THREADS = 1024;
-constexpr int PG_MOST_PAGES = 1 << 20;   // bound on max_pages: the new blocks of 1024 requests fit 31 bits
+constexpr int PG_MOST_PAGES = 1 << 20;   // bound on max_pages: the new blocks of 1024 requests are at most 2^30,
+constexpr int PG_MANY = (1 << 30) - 1;   // and those of all before them count as at most this: the sum fits 31 bits
 
 // Exclusive prefix sums over the CTA of a 64-bit and a 32-bit number per thread, and their totals.
 struct PgScan {
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(PG_THREADS) extend_pages_kernel(const __grid_c
   const int nf = max(0, min(*p.n_free, p.num_free));
   const int64_t t0 = p.n_tokens * blockIdx.x / gridDim.x, t1 = p.n_tokens * (blockIdx.x + 1) / gridDim.x;
   int64_t toks = 0;
-  int needs = 0;                         // (held at 2^30, more than any stack has)
+  int needs = 0;                         // (held at PG_MANY, as many as the largest stack has)
   for (int base = 0; base < p.B; base += PG_THREADS) {
     const int b = base + tid;
     int len = 0, add = 0;
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(PG_THREADS) extend_pages_kernel(const __grid_c
       }
     }
     toks += ta;
-    needs = min(needs + tn, 1 << 30);
+    needs = min(needs + tn, PG_MANY);
     __syncthreads();
   }
   if (map && !p.per_row)

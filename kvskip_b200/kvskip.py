@@ -352,6 +352,8 @@ def decode8(q, k, v, k_scale, v_scale, scale: float, *, lens: torch.Tensor | Non
     Returns dict(out of q's type, lse fp32 [B,Hq][, blk_max, blk_sum fp32 [B,Hq,nb]][, out_f32])."""
     if q.dim() == 4:
         q = q.squeeze(2)
+    if max_len is not None and max_len < 1:
+        raise ValueError("decode8: max_len >= 1")
     e = _EXT or ext()
     bi, bc = (None, None) if plan is None else (plan.block_idx, plan.block_cnt)
     out, lse, bmax, bsum, o32 = e.decode8(q, k, v, k_scale, v_scale, scale, lens, page_table, max_len or 0, bi, bc, stats,

@@ -134,6 +134,10 @@ def test_front_end_argument_errors():
         PagedKV8(1, 1, 1, 96, 64, "cpu")
     with pytest.raises(ValueError, match="at least 1"):
         PagedKV8(0, 1, 1, 64, 64, "cpu")
+    x = torch.zeros(1, 1, 64)
+    for bad in (0, -1):
+        with pytest.raises(ValueError, match="max_len"):
+            K.decode8(x, x, x, x, x, 1.0, max_len=bad)
 
 
 def test_debug_check_of_the_slot_list():
