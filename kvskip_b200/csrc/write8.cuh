@@ -329,6 +329,7 @@ write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_const
               if (r[u].row > 0) was[u] = *scale(r[u], c);
             }
           }
+          __syncwarp();                    // every lane of a row has the old scale before one of them stores the new one
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             uint32_t top = w8_top_finite(0u, x[u], inf);

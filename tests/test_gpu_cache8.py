@@ -533,6 +533,27 @@ def test_write8_many_tokens_of_many_requests(n):
         assert np.array_equal(s.cpu().numpy(), want_s) and np.array_equal(c.view(torch.uint8).cpu().numpy(), want_c)
 
 
+@pytest.mark.parametrize("n,D,kind", [(5, 128, "e4m3"), (300, 64, "e4m3"), (300, 128, "int8"), (2000, 128, "e4m3"),
+                                      (2000, 64, "int8"), (7500, 64, "e4m3")])
+def test_write8_single_tokens_that_grow_their_blocks(n, D, kind):
+    """One token each for n blocks, every one larger than what its block holds: all lanes of a row round their channels of
+    the earlier rows by the old scale, one of them stores the new one.  Every number of slots per warp, K and V unlike."""
+    Hkv, gen = 8, torch.Generator().manual_seed(n + D)
+    codes, scales = _pool(n, Hkv, D, kind, gen)
+    rows = torch.randint(1, 6, (n,), generator=gen)
+    slots = torch.randperm(n, generator=gen) * TILE + rows
+    big = torch.exp2(torch.randint(0, 9, (n, Hkv, 1), generator=gen).float()) * {"e4m3": 448.0, "int8": 127.0}[kind] / 4
+    x, y = (((torch.rand(n, Hkv, D, generator=gen) + 1) * big).to(torch.bfloat16) for _ in range(2))
+    k, ks = codes.to(DEV), scales.to(DEV)
+    v, vs = k.clone(), ks.clone()
+    K.write8(x.to(DEV), y.to(DEV), slots.to(DEV), k, v, ks, vs)
+    for t, c, s in ((x, k, ks), (y, v, vs)):
+        want_c, want_s = codes.view(torch.uint8).numpy().copy(), scales.numpy().copy()
+        R.write_ref(t.float().numpy(), slots.tolist(), want_c, want_s, kind)
+        assert (want_s > scales.numpy()).all()
+        assert np.array_equal(s.cpu().numpy(), want_s) and _same_codes(c.view(torch.uint8).cpu().numpy(), want_c, kind)
+
+
 # ------------------------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("inplace", [False, True])
 @pytest.mark.parametrize("B,hi,new_hi,pool,mode", [(1, 0, 1, 1.0, "packed"), (1, 130, 500, 1.0, "packed"),
