@@ -180,7 +180,9 @@ class PagedKV8:
         cache.release(done)                      # pages of finished requests go back
 
     Nothing here synchronises; a request that finds no page is refused (`granted`) and keeps its length.
-    `lens`, `table`, `free_pages` and `n_free` are device tensors that change in place."""
+    `lens`, `table`, `free_pages`, `n_free` and `granted` are device tensors that change in place, so that they say after a
+    replayed step what that step did.  `positions` (of the last extension's list) is another tensor for every call of `extend`;
+    after a step that `StepGraph` replays it is the one of the captured call."""
 
     def __init__(self, num_pages: int, B: int, Hkv: int, D: int, max_tokens: int, device,
                  dtype=torch.float8_e4m3fn):
@@ -199,7 +201,7 @@ class PagedKV8:
         self.table = torch.full((B, self.max_pages), -1, dtype=torch.int32, device=device)
         self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)   # page 0 on top
         self.n_free = torch.full((1,), num_pages, dtype=torch.int32, device=device)
-        self.granted = None
+        self.granted = torch.zeros(B, dtype=torch.bool, device=device)
         self.positions = None
         self._ones = torch.ones(B, dtype=torch.int32, device=device)
 
@@ -211,8 +213,8 @@ class PagedKV8:
         if n_tokens is None and per_row is None:
             per_row = 1
         r = K.extend_pages(self.lens, new, self.table, self.free_pages, self.n_free, n_tokens=n_tokens, per_row=per_row,
-                           lens_out=self.lens, n_free_out=self.n_free)
-        self.granted, self.positions = r["granted"], r["positions"]
+                           lens_out=self.lens, n_free_out=self.n_free, granted_out=self.granted)
+        self.positions = r["positions"]
         return r["slots"]
 
     def write(self, k_new: torch.Tensor, v_new: torch.Tensor, slots: torch.Tensor) -> None:
@@ -238,6 +240,12 @@ class PagedKV8:
 
     def note_replayed(self) -> None:
         pass
+
+    def graph_outputs(self):
+        return self.positions
+
+    def take_outputs(self, positions) -> None:
+        self.positions = positions
 
     def gather(self, b: int):
         """fp32 copies [Hkv,n,D] of request b's keys and values (tests, debugging; reads the length back)."""

@@ -952,7 +952,8 @@ void fill_pages(kvskip_pages_params& p, const at::Tensor& lens, const at::Tensor
 std::vector<at::Tensor> extend_pages(const at::Tensor& lens, const at::Tensor& new_, const at::Tensor& page_table,
                                      const at::Tensor& free_pages, const at::Tensor& n_free, int64_t n_tokens,
                                      int64_t per_row, const c10::optional<at::Tensor>& lens_out,
-                                     const c10::optional<at::Tensor>& n_free_out) {
+                                     const c10::optional<at::Tensor>& n_free_out,
+                                     const c10::optional<at::Tensor>& granted_out) {
   TORCH_CHECK(lens.is_cuda(), "lens: contiguous CUDA int32");
   const c10::cuda::CUDAGuard guard(lens.device());
   TORCH_CHECK(lens.dim() == 1 && new_.numel() == lens.numel(), "new: [B]");
@@ -967,7 +968,14 @@ std::vector<at::Tensor> extend_pages(const at::Tensor& lens, const at::Tensor& n
   NewTogether fresh;
   fresh.add(slots, shape, at::kLong);
   fresh.add(positions, shape, at::kInt);
-  fresh.add(granted, {B}, at::kBool);
+  if (granted_out.has_value()) {
+    granted = *granted_out;
+    TORCH_CHECK(granted.is_cuda() && granted.scalar_type() == at::kBool && granted.is_contiguous() && granted.numel() == B,
+                "granted_out: contiguous CUDA bool [B]");
+    same_device(lens, {&granted});
+  } else {
+    fresh.add(granted, {B}, at::kBool);
+  }
   fill_pages(p, lens, page_table, free_pages, n_free, lens_out, n_free_out, lo, fo, fresh);
   p.new_ = i32(new_, "new");
   same_device(lens, {&new_});
@@ -1086,7 +1094,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("slots"), py::arg("k"), py::arg("v"), py::arg("k_scale"), py::arg("v_scale"));
   m.def("extend_pages", &extend_pages, "pages and slots for the new tokens of every request", py::arg("lens"),
         py::arg("new"), py::arg("page_table"), py::arg("free_pages"), py::arg("n_free"), py::arg("n_tokens") = 0,
-        py::arg("per_row") = 0, py::arg("lens_out") = py::none(), py::arg("n_free_out") = py::none());
+        py::arg("per_row") = 0, py::arg("lens_out") = py::none(), py::arg("n_free_out") = py::none(),
+        py::arg("granted_out") = py::none());
   m.def("release_pages", &release_pages, "pages of finished requests back to the free stack", py::arg("done"),
         py::arg("lens"), py::arg("page_table"), py::arg("free_pages"), py::arg("n_free"),
         py::arg("lens_out") = py::none(), py::arg("n_free_out") = py::none());

@@ -38,7 +38,9 @@ class StepGraph:
 
     layers: objects with `graph_scalars()` (the host-decided scalars their next step would pass
     to the kernels) and `note_replayed()` (called once per replayed step so that their host-side
-    step counters keep up); `RefreshLayer` has both.  The return value of the captured `launch()`
+    step counters keep up); `RefreshLayer` has both.  A layer that keeps results of its launches as
+    attributes has `graph_outputs()` (asked right after a capture) and `take_outputs()` (handed them
+    after every replay, since calls outside the graph may have put others in their place).  The return value of the captured `launch()`
     (tensors in the graph's memory pool, rewritten by every replay) is returned by `step()`."""
 
     def __init__(self, launch, layers=(), eager: int = 1):
@@ -48,6 +50,7 @@ class StepGraph:
         self.graph = None
         self.result = None
         self.signature = None
+        self.kept = []
         self.captures = 0
         self.replays = 0
 
@@ -78,10 +81,13 @@ class StepGraph:
             with torch.cuda.graph(graph, capture_error_mode="thread_local"):
                 result = self.launch()          # recorded, not run; advances the layers' counters
             self.graph, self.result, self.signature = graph, result, sig
+            self.kept = [(layer, layer.graph_outputs()) for layer in self.layers if hasattr(layer, "graph_outputs")]
             self.captures += 1
         else:
             for layer in self.layers:
                 layer.note_replayed()
         self.graph.replay()
+        for layer, kept in self.kept:
+            layer.take_outputs(kept)
         self.replays += 1
         return self.result

@@ -400,7 +400,8 @@ def _check_runs(slots) -> None:
 
 
 def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | None = None, per_row: int | None = None,
-                 lens_out: torch.Tensor | None = None, n_free_out: torch.Tensor | None = None) -> dict:
+                 lens_out: torch.Tensor | None = None, n_free_out: torch.Tensor | None = None,
+                 granted_out: torch.Tensor | None = None) -> dict:
     """Pages and slots for `new` int32 [B] more tokens of requests that hold `lens` int32 [B] tokens, built on
     the device without a host synchronisation.  Not in the reference, whose caller counts on the host.
 
@@ -409,14 +410,14 @@ def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | N
     the slot list, or into what earlier requests left of the stack) is refused as a whole.
     Slots and positions: packed, request after request, in n_tokens places, or with per_row in a padded
     [B,per_row] list; -1 in places without a token.
-    Returns dict(slots int64, positions int32, granted bool [B], lens, n_free); the last two are new tensors unless
-    lens_out / n_free_out are given, which may be lens and n_free themselves."""
+    Returns dict(slots int64, positions int32, granted bool [B], lens, n_free); the last three are new tensors unless
+    granted_out / lens_out / n_free_out are given; the latter two may be lens and n_free themselves."""
     if (n_tokens is None) == (per_row is None):
         raise ValueError("extend_pages: either n_tokens (packed) or per_row (padded)")
     if per_row is not None and per_row < 1:
         raise ValueError("extend_pages: per_row >= 1")
     slots, positions, granted, lens2, n2 = (_EXT or ext()).extend_pages(lens, new, page_table, free_pages, n_free, n_tokens or 0,
-                                                              per_row or 0, lens_out, n_free_out)
+                                                              per_row or 0, lens_out, n_free_out, granted_out)
     return {"slots": slots, "positions": positions, "granted": granted, "lens": lens2, "n_free": n2}
 
 

@@ -597,6 +597,27 @@ def test_extend_and_release_pages(B, hi, new_hi, pool, mode, inplace):
     assert td.tolist() == want[4]
 
 
+def test_granted_and_positions_after_a_replay():
+    """A captured extension that the pool refuses says so in the cache's attributes, an eager one in between or not."""
+    cache = PagedKV8(3, 2, 1, 64, 256, DEV)
+    one = torch.ones(2, dtype=torch.int32, device=DEV)
+    step = StepGraph(lambda: cache.extend(one, per_row=1), [cache], eager=0)
+    step.step()
+    assert cache.granted.tolist() == [True, True] and cache.positions.flatten().tolist() == [0, 0]
+    cache.extend(torch.tensor([63, 63], dtype=torch.int32, device=DEV), n_tokens=126)       # both pages full, one left
+    assert cache.granted.tolist() == [True, True] and cache.lens.tolist() == [64, 64]
+    step.step()
+    assert cache.granted.tolist() == [True, False] and cache.positions.flatten().tolist() == [64, -1]
+    assert cache.lens.tolist() == [65, 64] and cache.n_free.tolist() == [0]
+    raw = torch.cuda.CUDAGraph()                                                             # a graph without StepGraph
+    with torch.cuda.graph(raw):
+        cache.extend(one, per_row=1)
+    cache.extend(torch.zeros(2, dtype=torch.int32, device=DEV), per_row=1)
+    assert cache.granted.tolist() == [True, True]
+    raw.replay()
+    assert cache.granted.tolist() == [True, False] and cache.lens.tolist() == [66, 64]
+
+
 # ------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("graph", [False, True], ids=["launches", "captured"])
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])

@@ -140,6 +140,49 @@ def test_front_end_argument_errors():
             K.decode8(x, x, x, x, x, 1.0, max_len=bad)
 
 
+def test_a_replayed_step_says_what_it_granted(monkeypatch):
+    """`granted` and `positions` of the cache are those of the replayed step, whatever was called in between."""
+    from kvskip_b200 import cache as C
+    from kvskip_b200 import graph as G
+
+    def extend_pages(lens, new, table, free, n_free, *, n_tokens=None, per_row=None, lens_out=None, n_free_out=None,
+                     granted_out=None):
+        granted = torch.empty(len(lens), dtype=torch.bool) if granted_out is None else granted_out
+        n = len(lens) * per_row if per_row else n_tokens
+        r = {"slots": torch.zeros(n, dtype=torch.int64), "positions": torch.full((n,), -1, dtype=torch.int32),
+             "granted": granted.fill_(True), "lens": lens, "n_free": n_free}
+        seen.append((r["granted"], r["positions"]))
+        return r
+
+    class Graph:
+        def replay(self):           # what the captured launch writes
+            seen[at[id(self)]][0].copy_(torch.tensor([True, False]))
+            seen[at[id(self)]][1].copy_(torch.tensor([7, -1]))
+
+    class Capture:
+        def __init__(self, g, **kw):
+            at[id(g)] = len(seen)
+
+        def __enter__(self):
+            pass
+
+        def __exit__(self, *a):
+            return False
+
+    seen, at = [], {}
+    monkeypatch.setattr(C.K, "extend_pages", extend_pages)
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", Graph)
+    monkeypatch.setattr(torch.cuda, "graph", Capture)
+    cache = PagedKV8(4, 2, 1, 64, 128, "cpu")
+    steps = [G.StepGraph(lambda: cache.extend(per_row=1), [cache], eager=0) for _ in range(2)]
+    for g in [steps[0], steps[1], steps[0], steps[0]]:
+        g.step()
+        assert cache.granted.tolist() == [True, False] and cache.positions.tolist() == [7, -1]
+        cache.extend(torch.tensor([3, 0], dtype=torch.int32), n_tokens=3)
+        assert cache.granted.tolist() == [True, True] and cache.positions.tolist() == [-1] * 3
+    assert steps[0].captures == steps[1].captures == 1
+
+
 def test_debug_check_of_the_slot_list():
     K._check_runs(torch.tensor([5, 6, 7, -1, 64, 65, 128, -1, -1, 200]))
     K._check_runs(torch.tensor([[62, 63], [64, 65]]))
