@@ -380,7 +380,7 @@ int kvskip_launch_write8(const kvskip_write8_params* p, void* stream);
  * table[b, 0..ceil(lens[b]/64)) and is to get new_[b] more (negative counts as 0); free_pages
  * [num_free] is a stack of the free pages, *n_free of them.  In the order of the requests, every request
  * that fits (into max_pages pages, into the slot list, and into what the earlier ones left of the stack;
- * one that needs no page always fits into the stack) is granted: its new blocks get pages from the top
+ * one that needs no page always fits into the stack, one without new tokens into any list) is granted: its new blocks get pages from the top
  * of the stack, written to the table, and its tokens their slot (page * 64 + row) and position.  Nothing
  * of a refused request changes; its slots are -1.  Once one request has found too few pages, no later one
  * gets a page.

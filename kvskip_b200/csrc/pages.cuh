@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(PG_THREADS) extend_pages_kernel(const __grid_c
     pg_scan(sh, at, nat, ta, tn);
     at += toks;
     nat += needs;
-    if (!p.per_row) fits = fits && at + add <= p.n_tokens;
+    if (!p.per_row) fits = fits && (add == 0 || at + add <= p.n_tokens);    // (no token: no place needed)
     const bool granted = fits && (need == 0 || nat + need <= nf);
     tok0[tid] = p.per_row ? static_cast<int64_t>(b) * p.per_row : at;
     need0[tid] = nat;

@@ -597,6 +597,22 @@ def test_extend_and_release_pages(B, hi, new_hi, pool, mode, inplace):
     assert td.tolist() == want[4]
 
 
+@pytest.mark.parametrize("B", [5, 1030])
+def test_extend_pages_grants_a_request_without_tokens_behind_a_full_list(B):
+    """The slot list has room for the first request only; what asks for no token needs no place in it and keeps running,
+    unless its length is beyond the table."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    lens, new = [10, 20, 30, 0, 200] + [70] * (B - 5), [4, 9, 0, -3, 0] + [0, 1] * ((B - 5) // 2) + [0] * ((B - 5) % 2)
+    table = torch.full((B, 2), -1, dtype=torch.int32, device=DEV)
+    table[:, 0] = torch.arange(B)
+    free = torch.arange(B, B + 8, dtype=torch.int32, device=DEV)
+    r = K.extend_pages(i32(lens), i32(new), table, free, i32([8]), n_tokens=6)
+    assert r["granted"].tolist() == [True, False, True, True, False] + [n == 0 for n in new[5:]]
+    assert r["slots"].tolist() == [10, 11, 12, 13, -1, -1] and r["positions"].tolist() == [10, 11, 12, 13, -1, -1]
+    assert r["lens"].tolist() == [14] + lens[1:] and r["n_free"].tolist() == [8]
+    assert torch.equal(table[:, 0].cpu(), torch.arange(B, dtype=torch.int32)) and (table[:, 1] == -1).all()
+
+
 def test_granted_and_positions_after_a_replay():
     """A captured extension that the pool refuses says so in the cache's attributes, an eager one in between or not."""
     cache = PagedKV8(3, 2, 1, 64, 256, DEV)
