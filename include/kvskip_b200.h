@@ -386,7 +386,8 @@ int kvskip_launch_write8(const kvskip_write8_params* p, void* stream);
  * gets a page.
  * Slot lists: per_row = 0, packed: the tokens of request 0, 1, ... one after the other, n_tokens entries;
  * per_row > 0: token i of request b at b * per_row + i (n_tokens = B * per_row).  Places without a token
- * get -1.  lens_out and n_free_out may be lens and n_free themselves; the stack is not written.
+ * get -1.  lens_out and n_free_out may be lens and n_free themselves; nothing else that is written may overlap anything
+ * that is read or written (refused); the stack is not written.
  * Limits: max_pages at most 2^20, num_free less than 2^30. */
 typedef struct kvskip_pages_params {
   const int32_t* lens;  /* [B] */

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "host.h"
 #include "common.cuh"
@@ -203,6 +204,29 @@ int check_pages(const kvskip_pages_params* p, const char* who) {
   return KVSKIP_OK;
 }
 
+// A stretch of memory that a call reads or writes; `same`: it may be that other one, exactly.
+struct Span {
+  const char* name;
+  const void* at;
+  int64_t bytes;
+  const void* same = nullptr;
+};
+// The blocks of a launch run at the same time: what one writes must not be what another reads or writes.
+int check_apart(const char* who, std::initializer_list<Span> written, std::initializer_list<Span> read) {
+  const auto meet = [](const Span& a, const Span& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return a.at && b.at && x < y + static_cast<uintptr_t>(b.bytes) && y < x + static_cast<uintptr_t>(a.bytes);
+  };
+  for (const Span* w = written.begin(); w != written.end(); ++w) {
+    for (const Span* o = w + 1; o != written.end(); ++o)
+      if (meet(*w, *o)) return fail(KVSKIP_E_ARG, "%s: %s and %s overlap", who, w->name, o->name);
+    for (const Span& r : read)
+      if (meet(*w, r) && !(w->same == r.at && w->at == r.at && w->bytes == r.bytes))
+        return fail(KVSKIP_E_ARG, "%s: %s and %s overlap", who, w->name, r.name);
+  }
+  return KVSKIP_OK;
+}
+
 }  // namespace
 
 namespace kvb_host {
@@ -289,6 +313,14 @@ int kvskip_launch_extend_pages(const kvskip_pages_params* p, void* stream) {
     return fail(KVSKIP_E_ARG, "extend_pages: new, granted, slots and positions are required");
   if (p->n_tokens < 0 || p->per_row < 0 || (p->per_row > 0 && p->n_tokens != static_cast<int64_t>(p->per_row) * p->B))
     return fail(KVSKIP_E_ARG, "extend_pages: n_tokens >= 0, and B * per_row of them in a padded list");
+  const int64_t B = p->B;
+  if (int rc = check_apart("extend_pages",
+                           {{"lens_out", p->lens_out, 4 * B, p->lens}, {"n_free_out", p->n_free_out, 4, p->n_free},
+                            {"table", p->table, 4 * B * p->max_pages}, {"slots", p->slots, 8 * p->n_tokens},
+                            {"positions", p->positions, 4 * p->n_tokens}, {"granted", p->granted, B}},
+                           {{"lens", p->lens, 4 * B}, {"n_free", p->n_free, 4}, {"new", p->new_, 4 * B},
+                            {"free_pages", p->free_pages, 4LL * p->num_free}}))
+    return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int grid = pages_grid(p->n_tokens);
   const bool in_place = p->lens_out == p->lens || p->n_free_out == p->n_free;
@@ -301,6 +333,13 @@ int kvskip_launch_extend_pages(const kvskip_pages_params* p, void* stream) {
 int kvskip_launch_release_pages(const kvskip_pages_params* p, void* stream) {
   if (int rc = check_pages(p, "release_pages")) return rc;
   if (!p->done) return fail(KVSKIP_E_ARG, "release_pages: done is required");
+  const int64_t B = p->B;
+  if (int rc = check_apart("release_pages",
+                           {{"lens_out", p->lens_out, 4 * B, p->lens}, {"n_free_out", p->n_free_out, 4, p->n_free},
+                            {"free_pages", p->free_pages, 4LL * p->num_free}},
+                           {{"lens", p->lens, 4 * B}, {"n_free", p->n_free, 4}, {"done", p->done, B},
+                            {"table", p->table, 4 * B * p->max_pages}}))
+    return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int grid = pages_grid(static_cast<int64_t>(p->B) * p->max_pages / 8);
   const bool in_place = p->lens_out == p->lens || p->n_free_out == p->n_free;

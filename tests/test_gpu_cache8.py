@@ -613,6 +613,17 @@ def test_extend_pages_grants_a_request_without_tokens_behind_a_full_list(B):
     assert torch.equal(table[:, 0].cpu(), torch.arange(B, dtype=torch.int32)) and (table[:, 1] == -1).all()
 
 
+def test_overlapping_tables_are_refused():
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    lens, new, table, free, n = i32([3, 70]), i32([1, 1]), i32([[0, -1], [1, 2]]), i32([5, 4, 3]), i32([3])
+    with pytest.raises(RuntimeError, match="lens_out and new overlap"):
+        K.extend_pages(lens, new, table, free, n, per_row=1, lens_out=new)
+    with pytest.raises(RuntimeError, match="lens_out and free_pages overlap"):
+        K.release_pages(i32([1, 0]).bool(), lens, table, free, n, lens_out=free[1:])
+    r = K.extend_pages(lens, lens, table, free, n, n_tokens=73, lens_out=lens, n_free_out=n)      # in place, twice the tokens
+    assert r["lens"].tolist() == [6, 70] and r["granted"].tolist() == [True, False] and n.tolist() == [3]
+
+
 def test_granted_and_positions_after_a_replay():
     """A captured extension that the pool refuses says so in the cache's attributes, an eager one in between or not."""
     cache = PagedKV8(3, 2, 1, 64, 256, DEV)

@@ -105,6 +105,27 @@ def test_pages_entries_refuse(lib, fn, change, text):
     assert text in lib.kvskip_last_error()
 
 
+_APART = dict(lens=0x10000, new_=0x20000, done=0x30000, table=0x40000, free_pages=0x50000, n_free=0x60000,
+              lens_out=0x70000, n_free_out=0x80000, slots=0x90000, positions=0xa0000, granted=0xb0000, n_tokens=9, B=7,
+              max_pages=4, num_free=9)
+
+
+@pytest.mark.parametrize("fn,change,text", [
+    ("extend_pages", dict(lens_out=0x20000), b"lens_out and new"), ("extend_pages", dict(lens_out=0x10004), b"lens_out and lens"),
+    ("extend_pages", dict(lens_out=0x10000, n_free_out=0x10000), b"lens_out and n_free_out"),
+    ("extend_pages", dict(n_free_out=0x10018), b"n_free_out and lens"), ("extend_pages", dict(table=0x50000 - 4), b"table and free_pages"),
+    ("extend_pages", dict(slots=0xa0000 - 64), b"slots and positions"), ("extend_pages", dict(granted=0x20000 + 27), b"granted and new"),
+    ("release_pages", dict(lens_out=0x50000 + 32), b"lens_out and free_pages"), ("release_pages", dict(done=0x70000), b"lens_out and done"),
+    ("release_pages", dict(free_pages=0x40000 + 108), b"free_pages and table"), ("release_pages", dict(n_free_out=0x10000), b"n_free_out and lens")])
+def test_pages_entries_refuse_outputs_in_inputs(lib, fn, change, text):
+    """The CTAs of one launch read all requests, and any of them may be the one that writes first."""
+    p = cabi.PagesParams()
+    for n, x in {**_APART, **change}.items():
+        setattr(p, n, x)
+    assert getattr(lib, f"kvskip_launch_{fn}")(ctypes.byref(p), None) == -1
+    assert text in lib.kvskip_last_error() and b"overlap" in lib.kvskip_last_error()
+
+
 def test_front_end_refuses_cpu_tensors():
     k = torch.zeros(3, 2, 64, 64, dtype=torch.float8_e4m3fn)
     s = torch.ones(3, 2)
