@@ -373,7 +373,8 @@ typedef struct kvskip_write8_params {
  * rounded to the new scale (exact for e4m3 short of its smallest values when the old scale is a power of
  * two).  Rows behind the run stay as they are.  All runs of one call go to different blocks: a run that
  * directly follows another one of the same block is skipped (status word 0x303), as is a slot
- * outside the cache (0x302); runs of one block further apart in the list race for it. */
+ * outside the cache (0x302); runs of one block further apart in the list race for it.  k, v and their scales
+ * are different memory, without strides of 0 (refused). */
 int kvskip_launch_write8(const kvskip_write8_params* p, void* stream);
 
 /* Page and slot tables from request lengths, on the device.  Request b holds lens[b] tokens in the pages

@@ -301,6 +301,12 @@ int kvskip_launch_write8(const kvskip_write8_params* p, void* stream) {
     return fail(KVSKIP_E_ARG, "write8: rows of k and v must be 8-byte aligned");
   if (p->Hkv > 65535 || p->n > 2147483647LL - 64 || (p->n + 3) / 4 * 2 * p->Hkv > 1073741823LL)
     return fail(KVSKIP_E_LIMIT, "write8: grid limits exceeded (tokens, heads)");
+  // K and V are written at the same time, and so are the heads and blocks of each
+  if (p->k == p->v || p->k_scale == p->v_scale) return fail(KVSKIP_E_ARG, "write8: k and v, or their scales, are the same memory");
+  const bool seqs = p->num_blocks > p->blocks, heads = p->Hkv > 1, blks = p->blocks > 1;
+  if ((seqs && (!p->k_sb || !p->v_sb || !p->ks_sb || !p->vs_sb)) || (heads && (!p->k_sh || !p->v_sh || !p->ks_sh || !p->vs_sh)) ||
+      (blks && (!p->ks_st || !p->vs_st)) || (p->tokens > 1 && (!p->k_st || !p->v_st)))
+    return fail(KVSKIP_E_ARG, "write8: a stride of 0 in k, v or their scales: several tokens or blocks in one place");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->kind == KVSKIP_KIND_E4M3)
     return p->D == 128 ? by_type<KVSKIP_KIND_E4M3, 128>(*p, s) : by_type<KVSKIP_KIND_E4M3, 64>(*p, s);

@@ -379,7 +379,7 @@ def write8(k_new, v_new, slots, k, v, k_scale, v_scale) -> None:
     afresh, whatever page and scale held before.  Infinities saturate; a NaN stays one in e4m3 and is 0 in int8.
     A slot outside the cache is skipped and sets the status word (`check_status`).  Two runs of one block in a call race
     for it unless they are neighbours (then the second is skipped, with the status word set); KVSKIP_CHECK_STATUS=1
-    refuses them."""
+    refuses them.  k and v, and k_scale and v_scale, are different memory, without strides of 0."""
     e = _EXT or ext()
     checked = e.check_wanted()
     if checked:

@@ -554,6 +554,24 @@ def test_write8_single_tokens_that_grow_their_blocks(n, D, kind):
         assert np.array_equal(s.cpu().numpy(), want_s) and _same_codes(c.view(torch.uint8).cpu().numpy(), want_c, kind)
 
 
+def test_write8_refuses_shared_memory():
+    x = torch.randn(2, 2, 64, device=DEV).to(torch.bfloat16)
+    k = torch.zeros(3, 2, 64, 64, dtype=torch.int8, device=DEV)
+    s = torch.ones(3, 2, device=DEV)
+    slots = torch.tensor([0, 64], device=DEV)
+    with pytest.raises(RuntimeError, match="same memory"):
+        K.write8(x, x, slots, k, k, s, s.clone())
+    with pytest.raises(RuntimeError, match="same memory"):
+        K.write8(x, x, slots, k, k.clone(), s, s)
+    with pytest.raises(RuntimeError, match="stride of 0"):
+        K.write8(x, x, slots, k, k.clone(), s[:1].clone().expand(3, 2), s)
+    both = torch.zeros(3, 2, 2, 64, 64, dtype=torch.int8, device=DEV)                              # K and V side by side
+    scales = torch.ones(3, 2, 2, device=DEV)
+    K.write8(x, 2 * x, slots, both[:, 0], both[:, 1], scales[:, 0], scales[:, 1])
+    K.write8(x, 2 * x, slots, k, (v := torch.zeros_like(k)), s, (t := torch.ones_like(s)))
+    assert torch.equal(both[:, 0], k) and torch.equal(both[:, 1], v) and torch.equal(scales[:, 0], s) and torch.equal(scales[:, 1], t)
+
+
 # ------------------------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("inplace", [False, True])
 @pytest.mark.parametrize("B,hi,new_hi,pool,mode", [(1, 0, 1, 1.0, "packed"), (1, 130, 500, 1.0, "packed"),

@@ -126,6 +126,23 @@ def test_pages_entries_refuse_outputs_in_inputs(lib, fn, change, text):
     assert text in lib.kvskip_last_error() and b"overlap" in lib.kvskip_last_error()
 
 
+@pytest.mark.parametrize("change,text", [
+    (dict(v=0x10000), b"same memory"), (dict(v_scale=0x30000), b"same memory"), (dict(vs_sb=0), b"stride of 0"),
+    (dict(k_sh=0), b"stride of 0"), (dict(ks_sh=0), b"stride of 0"), (dict(v_st=0), b"stride of 0"),
+    (dict(blocks=5, tokens=300, vs_st=0), b"stride of 0")])
+def test_write8_entry_refuses_shared_memory(lib, change, text):
+    """K and V, the heads and the blocks are written by different warps at the same time."""
+    p = cabi.Write8Params()
+    base = dict(k_new=0x50000, v_new=0x60000, kn_si=1024, kn_sh=128, vn_si=1024, vn_sh=128, n=4, inner=4, slots=0x70000,
+                k=0x10000, v=0x20000, k_sb=65536, k_sh=8192, k_st=128, v_sb=65536, v_sh=8192, v_st=128, k_scale=0x30000,
+                v_scale=0x40000, ks_sb=8, ks_sh=1, ks_st=1, vs_sb=8, vs_sh=1, vs_st=1, kind=0, Hkv=8, D=128, blocks=1,
+                tokens=64, num_blocks=10)
+    for n, x in {**base, **change}.items():
+        setattr(p, n, x)
+    assert lib.kvskip_launch_write8(ctypes.byref(p), None) == -1
+    assert text in lib.kvskip_last_error()
+
+
 def test_front_end_refuses_cpu_tensors():
     k = torch.zeros(3, 2, 64, 64, dtype=torch.float8_e4m3fn)
     s = torch.ones(3, 2)
