@@ -456,10 +456,12 @@ const char* kvskip_last_error(void);
 
 /* Reads (and clears) the current device's kernel status word after synchronising `stream`:
  * 0 if every bounded wait inside the kernels completed, otherwise the code of the first that
- * gave up (0x2xx / 0x4xx: a stage of a kernel's load ring; 0x300 / 0x301: a page table entry outside
- * the pool; 0x302 / 0x303: a slot outside the 8-bit cache, two runs of one block in a row; 0x6xx: a stage of
- * the 8-bit attention's loads; 0x310: plan's hand-over inside a cluster; 0x500 + peer, 0x510 + peer: the exchange between
- * GPUs).  Host-blocking; meant for tests and post-mortems, not for the hot path.  When the word is
+ * gave up (0x1xx / 0x2xx / 0x4xx and 0x308 to 0x37f: a stage of a kernel's load ring; 0x310 from plan: its hand-over
+ * inside a cluster; 0x500 + peer, 0x510 + peer: the exchange between GPUs; 0x600 to 0x61f: the read probe; 0x700 + warp,
+ * 0x720 + warp: a K or V tile of the 8-bit attention; 0x740 + warp: the values of an 8-bit write), or of an argument that
+ * pointed outside and was skipped (0x300 / 0x301: a page table entry outside the pool, in plan or append; 0x302: a slot
+ * outside the 8-bit cache; 0x303: two runs of one block next to each other).  The 8-bit cache's kernels keep a word of
+ * their own; where both are set, one call reports the other kernels' and the next call theirs.  Host-blocking; meant for tests and post-mortems, not for the hot path.  When the word is
  * non-zero the call also waits for the whole device and clears the split counters a kernel that
  * gave up may have left behind: no launch of this library may be in flight on another host thread. */
 int kvskip_device_status(void* stream, unsigned int* status);

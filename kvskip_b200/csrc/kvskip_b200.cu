@@ -1031,11 +1031,9 @@ int kvskip_device_status(void* stream, unsigned int* status) {
     void* ptr = nullptr;
     KVB_CUDA(cudaGetSymbolAddress(&ptr, g_split_done));
     KVB_CUDA(cudaMemset(ptr, 0, sizeof(int) * kMergeRegion * kMergeRegions));
+    return KVSKIP_OK;
   }
-  unsigned int st8 = 0;                       // the kernels of cache8.cu have a word of their own
-  if (int rc = kvb_host::cache8_status(&st8)) return rc;
-  if (!*status) *status = st8;
-  return KVSKIP_OK;
+  return kvb_host::cache8_status(status);     // the kernels of cache8.cu have a word of their own, left alone until reported
 }
 
 }  // extern "C"

@@ -119,7 +119,7 @@ vskip1_kernel(const kvskip_params p, const __grid_constant__ TmaMaps maps) {
       mbar_expect_tx(pro, Cfg::kTileBytes);
       tma_load_4d(sK, &maps.k, pro, 0, 0, h, b);
     }
-    mbar_wait(pro, 0, 0x300u);
+    mbar_wait(pro, 0, 0x308u);
     scores(reinterpret_cast<const uint16_t*>(sK), 0);
     __syncthreads();
     const float s0 = sS[warp * TILE + lane], s1 = sS[warp * TILE + lane + 32];

@@ -63,18 +63,26 @@ def ext():
 
 class DeviceWaitError(RuntimeError):
     """A bounded wait inside a kernel ran out (a load that never arrived, a peer GPU that never
-    flagged its rows).  `code` is the kernel's status word: 0x2xx / 0x3xx waits on this GPU's own
-    loads, 0x500 + r / 0x510 + r the exchange with rank r of a sequence-sharded step."""
+    flagged its rows), or a kernel skipped what one of its tables pointed to (0x300 to 0x303).  `code` is the
+    kernel's status word: 0x1xx to 0x4xx from 0x308 on, 0x6xx and 0x7xx waits on this GPU's own loads (0x700 / 0x720 + warp:
+    K / V of decode8, 0x740 + warp: write8), 0x500 + r / 0x510 + r the exchange with rank r of a sequence-sharded step."""
+
+    SKIPPED = {0x300: "a page table entry is outside the pool; the token was not read",
+               0x301: "a page table entry is outside the pool; the token was not written",
+               0x302: "a slot is outside the 8-bit cache; its token was not written",
+               0x303: "two runs of one block stand next to each other in the slot list; the second was not written"}
 
     def __init__(self, code: int, what: str):
-        super().__init__(f"{what}: a device-side wait gave up (status word {code:#x}); the results of that launch "
+        why = self.SKIPPED.get(code)
+        super().__init__(f"{what}: {why} (status word {code:#x})" if why else
+                         f"{what}: a device-side wait gave up (status word {code:#x}); the results of that launch "
                          "are incomplete")
         self.code = code
 
 
 def check_status(what: str = "kvskip") -> None:
     """Synchronise the current stream, read the kernels' status word and raise DeviceWaitError if a
-    wait timed out (the word is cleared).  Blocks the host: call it where a synchronisation is
+    wait timed out or a table pointed outside (the word is cleared).  Blocks the host: call it where a synchronisation is
     acceptable (end of a decode step, after a failed exchange), or set KVSKIP_CHECK_STATUS=1 to
     have every front-end call do it (debugging)."""
     code = int(ext().device_status())

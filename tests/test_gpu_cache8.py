@@ -554,6 +554,26 @@ def test_write8_single_tokens_that_grow_their_blocks(n, D, kind):
         assert np.array_equal(s.cpu().numpy(), want_s) and _same_codes(c.view(torch.uint8).cpu().numpy(), want_c, kind)
 
 
+def test_both_status_words_are_reported():
+    """A page outside the pool of the 16-bit cache, and a slot outside the 8-bit one: one call each."""
+    k = torch.zeros(2, 1, 64, 128, dtype=torch.bfloat16, device=DEV)
+    new = torch.ones(1, 1, 128, dtype=torch.bfloat16, device=DEV)
+    x = torch.ones(1, 1, 128, dtype=torch.bfloat16, device=DEV)
+    k8, s = torch.zeros(2, 1, 64, 128, dtype=torch.int8, device=DEV), torch.ones(2, 1, device=DEV)
+    for first in (True, False):
+        for paged in (first, not first):
+            if paged:
+                K.ext().append(k, k.clone(), new, new, 1, None, torch.full((1, 1), -1, dtype=torch.int32, device=DEV))
+            else:
+                K.write8(x, x, torch.tensor([128], device=DEV), k8, k8.clone(), s, s.clone())
+        with pytest.raises(K.DeviceWaitError, match="page table entry"):
+            K.check_status("append")
+        with pytest.raises(K.DeviceWaitError, match="slot is outside"):
+            K.check_status("write8")
+        K.check_status("nothing")
+    assert (k == 0).all() and (k8 == 0).all() and (s == 1).all()
+
+
 def test_write8_refuses_shared_memory():
     x = torch.randn(2, 2, 64, device=DEV).to(torch.bfloat16)
     k = torch.zeros(3, 2, 64, 64, dtype=torch.int8, device=DEV)

@@ -221,6 +221,14 @@ def test_a_replayed_step_says_what_it_granted(monkeypatch):
     assert steps[0].captures == steps[1].captures == 1
 
 
+def test_status_codes_say_what_happened():
+    for code, text in ((0x300, "page table"), (0x301, "page table"), (0x302, "slot is outside"), (0x303, "two runs")):
+        e = K.DeviceWaitError(code, "write8")
+        assert text in str(e) and hex(code) in str(e) and "wait" not in str(e) and e.code == code
+    for code in (0x200, 0x308, 0x501, 0x700, 0x741):
+        assert "wait gave up" in str(K.DeviceWaitError(code, "x"))
+
+
 def test_debug_check_of_the_slot_list():
     K._check_runs(torch.tensor([5, 6, 7, -1, 64, 65, 128, -1, -1, 200]))
     K._check_runs(torch.tensor([[62, 63], [64, 65]]))
