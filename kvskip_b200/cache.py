@@ -221,8 +221,9 @@ class PagedKV8:
         K.write8(k_new, v_new, slots, self.k, self.v, self.k_scale, self.v_scale)
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, new: torch.Tensor | None = None) -> None:
-        """One token per request, [B,Hkv,D] each; new (int32 [B] of 0 and 1) leaves rows out."""
-        slots = self.extend(new, per_row=1)
+        """One token per request, [B,Hkv,D] each.  new (int32 [B] of 0 and 1): the rows that get one, a row without a
+        request among them (which begins it); by default every row that holds a request, `lens[b] > 0`."""
+        slots = self.extend(self.lens.clamp(max=1) if new is None else new, per_row=1)
         self.write(k_new.unsqueeze(2), v_new.unsqueeze(2), slots)
 
     def release(self, done: torch.Tensor) -> None:

@@ -683,6 +683,30 @@ def test_granted_and_positions_after_a_replay():
     assert cache.granted.tolist() == [True, False] and cache.lens.tolist() == [66, 64]
 
 
+def test_append_leaves_rows_without_a_request_alone():
+    """After a release the row takes no page and no token until something is written for it."""
+    B, Hkv, D = 4, 2, 64
+    gen = torch.Generator().manual_seed(2)
+    cache = PagedKV8(9, B, Hkv, D, 256, DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    x = torch.randn(63 + 64 + 1, Hkv, D, generator=gen).to(torch.bfloat16).to(DEV)
+    cache.write(x, x, cache.extend(i32([63, 64, 0, 1]), n_tokens=128))
+    cache.release(torch.tensor([0, 1, 0, 0], dtype=torch.bool, device=DEV))
+    new = torch.randn(3, B, Hkv, D, generator=gen).to(torch.bfloat16).to(DEV)
+    codes, free = cache.k.view(torch.uint8).clone(), cache.free_pages.clone()
+    for t in range(3):
+        cache.append(new[t], new[t])
+    assert cache.lens.tolist() == [66, 0, 0, 4] and cache.n_free.tolist() == [6] and cache.granted.all()
+    mine = set(cache.table[0, :2].tolist() + cache.table[3, :1].tolist())
+    others = [p for p in range(9) if p not in mine]
+    assert len(mine) == 3 and torch.equal(cache.k.view(torch.uint8)[others], codes[others]) and torch.equal(cache.free_pages, free)
+    q = torch.randn(B, Hkv, D, generator=gen).to(torch.bfloat16).to(DEV)
+    r = cache.decode(q, 0.1)
+    assert (r["out"][1:3] == 0).all() and torch.isneginf(r["lse"][1:3]).all() and torch.isfinite(r["lse"][[0, 3]]).all()
+    cache.append(new[0], new[0], i32([0, 1, 0, 0]))                            # and a request that begins with one token
+    assert cache.lens.tolist() == [66, 1, 0, 4]
+
+
 # ------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("graph", [False, True], ids=["launches", "captured"])
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
