@@ -23,7 +23,8 @@
 // P (0..1 relative to its block's maximum) goes to the tensor cores as fp16 high + low parts, which hold
 // 22 bits of it: with G <= 4 the two parts share one instruction (columns 0-3 high, 4-7 low; the scores of a
 // head are computed in both, which costs nothing), else they are two instructions.  P is scaled by 2^13,
-// so that weights down to 2^-27 of the block's maximum are normal fp16 numbers.
+// so that weights down to 2^-27 of the block's maximum are normal fp16 numbers; the factor that brings a block's sums to the
+// running maximum takes the scaling out again, so that outputs up to the end of fp32 do not overflow on the way.
 #pragma once
 #include "common.cuh"
 #include "mma.cuh"
@@ -52,7 +53,7 @@ struct D8Cfg {
   static constexpr int kPiece = kCols * (D + 2);                     // floats of a piece: acc, m, l
 };
 
-constexpr float D8_PSCALE = 13.f;   // log2 of the scaling of P
+constexpr float D8_PSCALE = 13.f, D8_PUNSCALE = 1.f / 8192.f;   // log2 of the scaling of P, and what undoes it
 
 // The chunks of the work list.  Places in the list are costs: a block counts 4, and where heads are short (64 blocks on
 // average) and a warp has at least four blocks, the first block of a head D8_HEAD more (q is read and converted there, and
@@ -249,7 +250,7 @@ __device__ __forceinline__ void d8_store4(const kvskip_decode8_params& p, const 
   d8_store(p, hq, d0 + 2, x.z, x.w);
 }
 __device__ __forceinline__ float d8_lse(float m, float l) {
-  return l == 0.f ? -INFINITY : (m + log2f(l) - D8_PSCALE) * LN2;   // (a NaN sum stays one)
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;   // (a NaN sum stays one)
 }
 __device__ __forceinline__ float d8_safe(float m) { return m == -INFINITY ? 0.f : m; }
 // N pieces (maximum, sum, four channels) onto a sum relative to m_old, which becomes one relative to m.
@@ -631,7 +632,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
           mb[e] = quadcol_max(v);
           const float m_new = fmaxf(m_run[t][e], mb[e]), mu = d8_safe(m_new);
           alpha[t][e] = ex2(m_run[t][e] - mu);
-          beta[t][e] = ex2(mb[e] - mu);
+          beta[t][e] = ex2(mb[e] - mu) * D8_PUNSCALE;
           m_run[t][e] = m_new;
           rescale |= alpha[t][e] != 1.f;
         }
@@ -661,14 +662,13 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
           const float e0 = quadcol_sum(ls[0]), e1 = quadcol_sum(ls[1]);
           const int head = 8 * t + 2 * q4;
           if (g == 0 && blk >= 0 && blk < p.nb && (MODE != 0 || q4 < 2)) {
-            const float down = 1.f / 8192.f;
             if (head < G) {
               p.blk_max[(hq0 + head) * p.nb + blk] = mb[0] * LN2;
-              p.blk_sum[(hq0 + head) * p.nb + blk] = e0 * down;
+              p.blk_sum[(hq0 + head) * p.nb + blk] = e0 * D8_PUNSCALE;
             }
             if (head + 1 < G) {
               p.blk_max[(hq0 + head + 1) * p.nb + blk] = mb[1] * LN2;
-              p.blk_sum[(hq0 + head + 1) * p.nb + blk] = e1 * down;
+              p.blk_sum[(hq0 + head + 1) * p.nb + blk] = e1 * D8_PUNSCALE;
             }
           }
         }

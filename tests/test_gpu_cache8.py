@@ -245,6 +245,28 @@ def test_decode8_extreme_values(kind):
     _check(_run(_dev(c), stats=True), ref, D, c["nb"], torch.bfloat16)
 
 
+@pytest.mark.parametrize("G,T", [(4, 700), (8, 700), (16, 700), (4, 40000)])
+def test_decode8_values_near_the_end_of_the_type(G, T):
+    """Values of 2^115, as bf16 has them: the sums of hundreds of tokens stay inside fp32, whose end is 2^128.  And what
+    `write8` made of such values."""
+    lens, Hkv, D = [T, 130], 2, 128
+    c = _case(lens, Hkv, G, D, "e4m3", torch.bfloat16, "contiguous", seed=G)
+    c["vs"] *= 2.0 ** 112 if T < 1000 else 2.0 ** 106
+    ref = R.decode_f64(c["q"], _cpu(c["k"]), _cpu(c["v"]), c["ks"], c["vs"], c["scale"], lens)
+    assert float(ref["mag"].max()) * T < 2.0 ** 127
+    r = _run(_dev(c), stats=True)
+    assert torch.isfinite(r["out"]).all()
+    _check(r, ref, D, c["nb"], torch.bfloat16)
+    cache = PagedKV8(4, 1, Hkv, D, 256, DEV)
+    x = torch.randn(200, Hkv, D, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+    big = (x.float() * 2.0 ** 116).to(torch.bfloat16)
+    cache.write(x, big, cache.extend(torch.tensor([200], dtype=torch.int32, device=DEV), n_tokens=200))
+    r = cache.decode(c["q"][:1].to(DEV), c["scale"], out_f32=True)
+    ref = R.decode_f64(c["q"][:1], _cpu(cache.k), _cpu(cache.v), cache.k_scale.cpu(), cache.v_scale.cpu(), c["scale"], [200],
+                       cache.table.cpu())
+    _check(r, ref, D, 4, torch.bfloat16)
+
+
 def test_decode8_nan_stays_in_its_row():
     lens, Hkv, G, D = [300, 300], 2, 4, 128
     c = _case(lens, Hkv, G, D, "e4m3", torch.bfloat16, "paged", seed=4)
