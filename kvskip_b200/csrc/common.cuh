@@ -85,6 +85,17 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
   return false;
 }
 
+// The same for a warp whose lanes go on together: one that gives up takes the others along (the instructions behind the
+// wait are executed by the whole warp).
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, unsigned int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+// A copy that is still on its way when a kernel gives up: waited for, within the same bound, before the kernel leaves.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  for (uint32_t it = 0; it < SPIN_LIMIT; ++it)
+    if (mbar_try_wait(bar, parity)) return;
+}
+
 // ---- thread-block clusters ------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

@@ -578,7 +578,10 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
       };
       const int lrow = lane & 7, lmat = lane >> 3;
 
-      if (!mbar_wait(&bar[0], phase, 0x700u + warp)) break;
+      if (!mbar_wait_warp(&bar[0], phase, 0x700u + warp)) {
+        mbar_drain(&bar[1], phase);
+        break;
+      }
       // ---- S^T = K Q^T: 4 tiles of 16 tokens x 8 columns
       float sc[CT][4][4];
 #pragma unroll
@@ -679,7 +682,10 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
         }
       }
 
-      if (!mbar_wait(&bar[1], phase, 0x720u + warp)) break;
+      if (!mbar_wait_warp(&bar[1], phase, 0x720u + warp)) {
+        if (!last || next_n > 0) mbar_drain(&bar[0], phase ^ 1);
+        break;
+      }
       if (KIND == KVSKIP_KIND_E4M3 && tok < TILE) {
         // V rows behind the length: their weights are zero, but zero times a NaN code is not (int8 has none)
         for (int o = tok * D + lane * 16; o < TILE * D; o += 512) *reinterpret_cast<uint4*>(vstage + o) = make_uint4(0u, 0u, 0u, 0u);

@@ -258,7 +258,7 @@ write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_const
           uint32_t top = 0;
           const uint4* mine = reinterpret_cast<const uint4*>(stage) + lane;     // row r0, then every RPW-th
           if (staged) {
-            if (!mbar_wait(bar, phase, 0x740u + warp)) return;
+            if (!mbar_wait_warp(bar, phase, 0x740u + warp)) return;
             phase ^= 1;
             const int full = r.n / RPW;
             int q = 0;
