@@ -167,9 +167,9 @@ int launch_write8(const kvskip_write8_params& p, cudaStream_t s) {
   kvb::W8Maps maps{};
   const bool tma = token_map(&maps.k, p, p.k_new, p.kn_so, p.kn_si, p.kn_sh) &&
                    token_map(&maps.v, p, p.v_new, p.vn_so, p.vn_si, p.vn_sh);
-  const int64_t jobs = (p.n + CHUNK - 1) / CHUNK * 2 * p.Hkv;        // one pair each
+  const int64_t jobs = (p.n + CHUNK - 1) / CHUNK * 2 * p.Hkv;
   const int64_t ctas = std::min<int64_t>((jobs + Cfg::kWarps - 1) / Cfg::kWarps, kvb_host::num_sms() * (227 * 1024 / Cfg::kSmem));
-  KVB_CUDA(launch(kernel, dim3(static_cast<unsigned>(ctas)), Cfg::kThreads, Cfg::kSmem, s, p, maps, 1, static_cast<int>(jobs),
+  KVB_CUDA(launch(kernel, dim3(static_cast<unsigned>(ctas)), Cfg::kThreads, Cfg::kSmem, s, p, maps, static_cast<int>(jobs),
                   tma ? 1 : 0));
   return KVSKIP_OK;
 }

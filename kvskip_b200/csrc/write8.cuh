@@ -9,7 +9,7 @@
 //
 // What bounds it: 2 bytes read and 1 written per element: HBM for prompts, the chain slot -> scale so far -> codes for a
 // decode step.  A warp takes the runs (tokens of one block, consecutive rows) that begin among CHUNK entries of the
-// slot list, for `items` of the 2 Hkv (head, K or V) pairs, and needs no other warp: it looks at the slots with ballots,
+// slot list, for one of the 2 Hkv (head, K or V) pairs, and needs no other warp: it looks at the slots with ballots,
 // brings a run's values into its own 64 rows of shared memory with TMA, reads them there once for the maximum and
 // once for the codes.  Runs of one token, those of a decode step, are read from global memory directly, two or four an
 // instruction and four or eight at once.
@@ -115,11 +115,11 @@ struct W8Cfg {
   static constexpr int kSmem = kWarps * kStage + 128;
 };
 
-// tma: the tensor maps are valid (all strides positive); jobs: chunks of the slot list times groups of `items` pairs.
+// tma: the tensor maps are valid (all strides positive); jobs: chunks of the slot list times pairs.
 template <int KIND, int D, int CHUNK, bool F16>
 __global__ void __launch_bounds__(W8Cfg<D, CHUNK>::kThreads, 1)
-write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_constant__ W8Maps maps, const int items,
-              const int jobs, const int tma) {
+write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_constant__ W8Maps maps, const int jobs,
+              const int tma) {
   using Cfg = W8Cfg<D, CHUNK>;
   constexpr int NW = Cfg::kWarps;
   constexpr int LPR = D / 8, RPW = 32 / LPR;        // lanes of a row, 8 values each; rows of an instruction
@@ -136,12 +136,12 @@ write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_const
   pdl_wait_prior();
   pdl_launch_dependents();
 
-  const int n = static_cast<int>(p.n), groups = (2 * p.Hkv + items - 1) / items;
+  const int n = static_cast<int>(p.n), pairs = 2 * p.Hkv;
   const uint32_t inner = static_cast<uint32_t>(p.inner);
   const int ch = lane % LPR, r0 = lane / LPR;
   uint32_t phase = 0;
   auto read_slots = [&](const int job, int64_t (&s)[WORDS], int64_t& prev) {
-    const int i0 = job / groups * CHUNK;
+    const int i0 = job / pairs * CHUNK;
     prev = -1;
     if (lane == 0 && i0 > 0) prev = p.slots[i0 - 1];
 #pragma unroll
@@ -157,8 +157,9 @@ write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_const
   if (job < jobs) read_slots(job, ahead, ahead_prev);
 
   for (; job < jobs; job += step) {
-    const int i0 = job / groups * CHUNK;
-    const int c0 = job % groups * items, c1 = min(c0 + items, 2 * p.Hkv);    // pairs: K heads, then V heads
+    const int i0 = job / pairs * CHUNK;
+    const int c = job % pairs;             // K heads, then V heads
+    const bool v = c >= p.Hkv;
     int64_t slot[WORDS], last = ahead_prev;
 #pragma unroll
     for (int k = 0; k < WORDS; ++k) slot[k] = ahead[k];
@@ -176,7 +177,7 @@ write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_const
     for (int k = 0; k < WORDS; ++k) {
       const bool in = k * 32 + lane < CHUNK;
       if (outside(slot[k])) {
-        if (in && c0 == 0) atomicCAS(&g_status, 0u, 0x302u);
+        if (in && c == 0) atomicCAS(&g_status, 0u, 0x302u);
         slot[k] = -1;
       }
       int64_t before = __shfl_up_sync(0xffffffffu, slot[k], 1);
@@ -185,7 +186,7 @@ write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_const
       const bool some = slot[k] >= 0;
       const bool cont = some && before >= 0 && slot[k] == before + 1 && (slot[k] & (TILE - 1)) != 0;
       const bool twice = some && !cont && before >= 0 && (slot[k] >> 6) == (before >> 6);   // a second run of the block
-      if (twice && in && c0 == 0) atomicCAS(&g_status, 0u, 0x303u);
+      if (twice && in && c == 0) atomicCAS(&g_status, 0u, 0x303u);
       brk[k] = __ballot_sync(0xffffffffu, !cont);
       lead[k] = __ballot_sync(0xffffffffu, some && !cont && !twice && in);
     }
@@ -215,23 +216,23 @@ write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_const
       if (p.blocks > 1) r.blk = r.seq % p.blocks, r.seq /= p.blocks;
       return r;
     };
-    auto source = [&](const uint32_t at, const int c) -> const uint16_t* {    // values of one token
+    auto source = [&](const uint32_t at) -> const uint16_t* {    // values of one token
       const uint32_t o = inner == static_cast<uint32_t>(n) ? 0u : at / inner, in = at - o * inner;
-      return c >= p.Hkv ? p.v_new + o * p.vn_so + in * p.vn_si + (c - p.Hkv) * p.vn_sh : p.k_new + o * p.kn_so + in * p.kn_si + c * p.kn_sh;
+      return v ? p.v_new + o * p.vn_so + in * p.vn_si + (c - p.Hkv) * p.vn_sh : p.k_new + o * p.kn_so + in * p.kn_si + c * p.kn_sh;
     };
-    auto codes = [&](const Run& r, const int c) -> uint8_t* {
-      return c >= p.Hkv ? p.v + r.seq * p.v_sb + (c - p.Hkv) * p.v_sh + (r.blk * TILE + r.row) * p.v_st
-                        : p.k + r.seq * p.k_sb + c * p.k_sh + (r.blk * TILE + r.row) * p.k_st;
+    auto codes = [&](const Run& r) -> uint8_t* {
+      return v ? p.v + r.seq * p.v_sb + (c - p.Hkv) * p.v_sh + (r.blk * TILE + r.row) * p.v_st
+               : p.k + r.seq * p.k_sb + c * p.k_sh + (r.blk * TILE + r.row) * p.k_st;
     };
-    auto scale = [&](const Run& r, const int c) -> float* {
-      return c >= p.Hkv ? p.v_scale + r.seq * p.vs_sb + (c - p.Hkv) * p.vs_sh + r.blk * p.vs_st
-                        : p.k_scale + r.seq * p.ks_sb + c * p.ks_sh + r.blk * p.ks_st;
+    auto scale = [&](const Run& r) -> float* {
+      return v ? p.v_scale + r.seq * p.vs_sb + (c - p.Hkv) * p.vs_sh + r.blk * p.vs_st
+               : p.k_scale + r.seq * p.ks_sb + c * p.ks_sh + r.blk * p.ks_st;
     };
     auto usable = [](const float o) { return o > 0.f && o <= 3.402823466e38f ? o : W8_MIN_SCALE; };
     // rows before the run, rounded to the larger scale
-    auto again = [&](const Run& r, const int c, const float ratio, const int row0, const int rows) {
-      const int64_t st = c >= p.Hkv ? p.v_st : p.k_st;
-      w8_again<KIND>(codes(r, c) - r.row * st + 8 * ch, st, row0, r.row, rows, ratio);
+    const int64_t st = v ? p.v_st : p.k_st;
+    auto again = [&](const Run& r, const float ratio, const int row0, const int rows) {
+      w8_again<KIND>(codes(r) - r.row * st + 8 * ch, st, row0, r.row, rows, ratio);
     };
     auto put = [&](uint8_t* y, const uint4 x, const float s, const float inv) {
       *reinterpret_cast<uint2*>(y) = inv != 0.f ? w8_codes8<KIND, F16>(x, inv) : w8_codes8_div<KIND, F16>(x, s);
@@ -244,106 +245,101 @@ write8_kernel(const __grid_constant__ kvskip_write8_params p, const __grid_const
         const Run r = open(k, __ffs(rest) - 1);
         const uint32_t at = i0 + r.i, o = inner == static_cast<uint32_t>(n) ? 0u : at / inner, in = at - o * inner;
         const bool staged = tma && in + r.n <= inner;      // (a run may go on in the next row of a padded list)
-        for (int c = c0; c < c1; ++c) {
-          const bool v = c >= p.Hkv;
-          float was = W8_MIN_SCALE;
-          if (r.row > 0) was = *scale(r, c);
-          if (staged && lane == 0) {
-            const int boxes = (r.n + 15) / 16;
-            mbar_expect_tx(bar, boxes * 16 * D * 2);
-            for (int x = 0; x < boxes; ++x)
-              tma_load_4d(stage + x * 16 * D * 2, v ? &maps.v : &maps.k, bar, 0, in + 16 * x, v ? c - p.Hkv : c, o);
-          }
-          was = usable(was);
-          uint32_t top = 0;
-          const uint4* mine = reinterpret_cast<const uint4*>(stage) + lane;     // row r0, then every RPW-th
-          if (staged) {
-            if (!mbar_wait_warp(bar, phase, 0x740u + warp)) return;
-            phase ^= 1;
-            const int full = r.n / RPW;
-            int q = 0;
-            for (; q + 8 <= full; q += 8)
-#pragma unroll
-              for (int u = 0; u < 8; ++u) top = w8_top(top, mine[(q + u) * 32]);
-            for (; q * RPW + r0 < r.n; ++q) top = w8_top(top, mine[q * 32]);
-            if (__any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) >= inf)) {
-              top = 0;
-              for (q = 0; q * RPW + r0 < r.n; ++q) top = w8_top_finite(top, mine[q * 32], inf);
-            }
-          } else {
-            for (int q = r0; q < r.n; q += RPW)
-              top = w8_top_finite(top, *reinterpret_cast<const uint4*>(source(at + q, c) + 8 * ch), inf);
-          }
-          top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
-          const float s = fmaxf(was, w8_scale<KIND, F16>(top)), inv = w8_inverse(s);
-          const int64_t st = v ? p.v_st : p.k_st;
-          uint8_t* y = codes(r, c) + r0 * st + 8 * ch;
-          if (staged && inv != 0.f) {
-            const int full = r.n / RPW;
-            int q = 0;
-            for (; q + 4 <= full; q += 4, y += 4 * RPW * st)
-#pragma unroll
-              for (int u = 0; u < 4; ++u) *reinterpret_cast<uint2*>(y + u * RPW * st) = w8_codes8<KIND, F16>(mine[(q + u) * 32], inv);
-            for (; q * RPW + r0 < r.n; ++q, y += RPW * st) *reinterpret_cast<uint2*>(y) = w8_codes8<KIND, F16>(mine[q * 32], inv);
-          } else {
-            for (int q = r0; q < r.n; q += RPW, y += RPW * st)
-              put(y, staged ? mine[(q - r0) / RPW * 32] : *reinterpret_cast<const uint4*>(source(at + q, c) + 8 * ch), s, inv);
-          }
-          if (r.row > 0 && s > was) again(r, c, __fdiv_rn(was, s), r0, RPW);
-          __syncwarp();                    // the stage has been read, and the old scale by every lane
-          if (lane == 0) *scale(r, c) = s;
+        float was = W8_MIN_SCALE;
+        if (r.row > 0) was = *scale(r);
+        if (staged && lane == 0) {
+          const int boxes = (r.n + 15) / 16;
+          mbar_expect_tx(bar, boxes * 16 * D * 2);
+          for (int x = 0; x < boxes; ++x)
+            tma_load_4d(stage + x * 16 * D * 2, v ? &maps.v : &maps.k, bar, 0, in + 16 * x, v ? c - p.Hkv : c, o);
         }
+        was = usable(was);
+        uint32_t top = 0;
+        const uint4* mine = reinterpret_cast<const uint4*>(stage) + lane;     // row r0, then every RPW-th
+        if (staged) {
+          if (!mbar_wait_warp(bar, phase, 0x740u + warp)) return;
+          phase ^= 1;
+          const int full = r.n / RPW;
+          int q = 0;
+          for (; q + 8 <= full; q += 8)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) top = w8_top(top, mine[(q + u) * 32]);
+          for (; q * RPW + r0 < r.n; ++q) top = w8_top(top, mine[q * 32]);
+          if (__any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) >= inf)) {
+            top = 0;
+            for (q = 0; q * RPW + r0 < r.n; ++q) top = w8_top_finite(top, mine[q * 32], inf);
+          }
+        } else {
+          for (int q = r0; q < r.n; q += RPW)
+            top = w8_top_finite(top, *reinterpret_cast<const uint4*>(source(at + q) + 8 * ch), inf);
+        }
+        top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+        const float s = fmaxf(was, w8_scale<KIND, F16>(top)), inv = w8_inverse(s);
+        uint8_t* y = codes(r) + r0 * st + 8 * ch;
+        if (staged && inv != 0.f) {
+          const int full = r.n / RPW;
+          int q = 0;
+          for (; q + 4 <= full; q += 4, y += 4 * RPW * st)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) *reinterpret_cast<uint2*>(y + u * RPW * st) = w8_codes8<KIND, F16>(mine[(q + u) * 32], inv);
+          for (; q * RPW + r0 < r.n; ++q, y += RPW * st) *reinterpret_cast<uint2*>(y) = w8_codes8<KIND, F16>(mine[q * 32], inv);
+        } else {
+          for (int q = r0; q < r.n; q += RPW, y += RPW * st)
+            put(y, staged ? mine[(q - r0) / RPW * 32] : *reinterpret_cast<const uint4*>(source(at + q) + 8 * ch), s, inv);
+        }
+        if (r.row > 0 && s > was) again(r, __fdiv_rn(was, s), r0, RPW);
+        __syncwarp();                    // the stage has been read, and the old scale by every lane
+        if (lane == 0) *scale(r) = s;
       }
 
     // ---- runs of one token: lanes r0 = 0 .. RPW - 1 take one each, kBatch / RPW of them at once
     constexpr int U = Cfg::kBatch / RPW;
-    for (int c = c0; c < c1; ++c)
 #pragma unroll
-      for (int k = 0; k < (CHUNK + 31) / 32; ++k)
-        for (uint32_t rest = single[k]; rest;) {
-          Run r[U];
-          uint4 x[U];
-          float was[U];
+    for (int k = 0; k < (CHUNK + 31) / 32; ++k)
+      for (uint32_t rest = single[k]; rest;) {
+        Run r[U];
+        uint4 x[U];
+        float was[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            r[u].i = -1;
+        for (int u = 0; u < U; ++u) {
+          r[u].i = -1;
 #pragma unroll
-            for (int m = 0; m < RPW; ++m) {
-              const int bit = rest ? __ffs(rest) - 1 : 0;
-              const int64_t s = __shfl_sync(0xffffffffu, slot[k], bit);
-              if (m == r0 && rest) {
-                r[u].i = k * 32 + bit, r[u].n = 1;
-                r[u].row = static_cast<int>(s & (TILE - 1));
-                r[u].seq = s >> 6, r[u].blk = 0;
-                if (p.blocks > 1) r[u].blk = r[u].seq % p.blocks, r[u].seq /= p.blocks;
-              }
-              rest &= rest - 1;
+          for (int m = 0; m < RPW; ++m) {
+            const int bit = rest ? __ffs(rest) - 1 : 0;
+            const int64_t s = __shfl_sync(0xffffffffu, slot[k], bit);
+            if (m == r0 && rest) {
+              r[u].i = k * 32 + bit, r[u].n = 1;
+              r[u].row = static_cast<int>(s & (TILE - 1));
+              r[u].seq = s >> 6, r[u].blk = 0;
+              if (p.blocks > 1) r[u].blk = r[u].seq % p.blocks, r[u].seq /= p.blocks;
             }
-          }
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            x[u] = make_uint4(0u, 0u, 0u, 0u);
-            was[u] = W8_MIN_SCALE;
-            if (r[u].i >= 0) {
-              x[u] = *reinterpret_cast<const uint4*>(source(i0 + r[u].i, c) + 8 * ch);
-              if (r[u].row > 0) was[u] = *scale(r[u], c);
-            }
-          }
-          __syncwarp();                    // every lane of a row has the old scale before one of them stores the new one
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            uint32_t top = w8_top_finite(0u, x[u], inf);
-            top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-            for (int d = LPR / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-            if (r[u].i >= 0) {
-              const float old = usable(was[u]), s = fmaxf(old, w8_scale<KIND, F16>(top));
-              put(codes(r[u], c) + 8 * ch, x[u], s, w8_inverse(s));
-              if (r[u].row > 0 && s > old) again(r[u], c, __fdiv_rn(old, s), 0, 1);
-              if (ch == 0) *scale(r[u], c) = s;
-            }
+            rest &= rest - 1;
           }
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          x[u] = make_uint4(0u, 0u, 0u, 0u);
+          was[u] = W8_MIN_SCALE;
+          if (r[u].i >= 0) {
+            x[u] = *reinterpret_cast<const uint4*>(source(i0 + r[u].i) + 8 * ch);
+            if (r[u].row > 0) was[u] = *scale(r[u]);
+          }
+        }
+        __syncwarp();                    // every lane of a row has the old scale before one of them stores the new one
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          uint32_t top = w8_top_finite(0u, x[u], inf);
+          top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+          for (int d = LPR / 2; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+          if (r[u].i >= 0) {
+            const float old = usable(was[u]), s = fmaxf(old, w8_scale<KIND, F16>(top));
+            put(codes(r[u]) + 8 * ch, x[u], s, w8_inverse(s));
+            if (r[u].row > 0 && s > old) again(r[u], __fdiv_rn(old, s), 0, 1);
+            if (ch == 0) *scale(r[u]) = s;
+          }
+        }
+      }
   }
 }
 
