@@ -215,7 +215,7 @@ struct Span {
 int check_apart(const char* who, std::initializer_list<Span> written, std::initializer_list<Span> read) {
   const auto meet = [](const Span& a, const Span& b) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
-    return a.at && b.at && x < y + static_cast<uintptr_t>(b.bytes) && y < x + static_cast<uintptr_t>(a.bytes);
+    return a.at && b.at && a.bytes > 0 && b.bytes > 0 && x < y + static_cast<uintptr_t>(b.bytes) && y < x + static_cast<uintptr_t>(a.bytes);
   };
   for (const Span* w = written.begin(); w != written.end(); ++w) {
     for (const Span* o = w + 1; o != written.end(); ++o)

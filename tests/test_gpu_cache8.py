@@ -296,6 +296,20 @@ def test_decode8_lists_without_a_token_and_negative_scale(G, bound):
     assert (r["out_f32"][0, :G] == 0).all() and torch.isneginf(r["lse"][0, :G]).all()
 
 
+@pytest.mark.parametrize("G,bound", [(4, 4), (4, 4000), (16, 4), (8, 4000)])
+def test_decode8_batch_without_a_token(G, bound):
+    """Every form of the launch: nothing is read, every output written."""
+    c = _dev(_case([0, 0, 0], 2, G, 128, "e4m3", torch.bfloat16, "paged", seed=1, T=bound * TILE))
+    junk = torch.full((1 << 22,), math.nan, device=DEV)
+    del junk                                                          # (the outputs' memory)
+    r = _run(c, stats=True)
+    assert (r["out"] == 0).all() and (r["out_f32"] == 0).all() and torch.isneginf(r["lse"]).all()
+    assert torch.isneginf(r["blk_max"]).all() and (r["blk_sum"] == 0).all()
+    e = K.extend_pages(c["lens"], c["lens"], c["table"], torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV),
+                       n_tokens=0)
+    assert e["granted"].all() and e["slots"].numel() == 0 and e["lens"].tolist() == [0, 0, 0]
+
+
 def test_c_entry_points_give_the_same_bits():
     from kvskip_b200.cabi import CAbi
     lib = CAbi()

@@ -126,6 +126,15 @@ def test_pages_entries_refuse_outputs_in_inputs(lib, fn, change, text):
     assert text in lib.kvskip_last_error() and b"overlap" in lib.kvskip_last_error()
 
 
+def test_an_empty_slot_list_overlaps_nothing(lib):
+    """Refused for what comes next: the zero-sized lists point into `new`, which does not matter."""
+    p = cabi.PagesParams()
+    for n, x in {**_APART, "slots": 0x20004, "positions": 0x20004, "n_tokens": 0, "granted": 0x20001}.items():
+        setattr(p, n, x)
+    assert lib.kvskip_launch_extend_pages(ctypes.byref(p), None) == -1
+    assert b"granted and new overlap" in lib.kvskip_last_error()
+
+
 @pytest.mark.parametrize("change,text", [
     (dict(v=0x10000), b"same memory"), (dict(v_scale=0x30000), b"same memory"), (dict(vs_sb=0), b"stride of 0"),
     (dict(k_sh=0), b"stride of 0"), (dict(ks_sh=0), b"stride of 0"), (dict(v_st=0), b"stride of 0"),
