@@ -298,7 +298,7 @@ int kvskip_launch_append(uint16_t* k, uint16_t* v, int64_t sb, int64_t sh, int64
  * kind 1: int8 (codes -127..127).  D is 64 or 128.
  * Paged form: codes uint8 [num_pages,Hkv,64,D], scales [num_pages,Hkv], a page table; contiguous
  * form: codes [B,Hkv,T,D], scales [B,Hkv,ceil(T/64)].  D contiguous, all other strides free (code
- * strides multiples of 16 bytes, 16-byte aligned base).  The entry points are stateless: no memory is
+ * strides positive multiples of 16 bytes, 16-byte aligned base).  The entry points are stateless: no memory is
  * shared between calls, so calls on different streams, and graphs captured from them, are independent
  * as long as their buffers are. */
 #define KVSKIP_KIND_E4M3 0

@@ -232,6 +232,9 @@ class PagedKV8:
 
     def decode(self, q, scale: float, plan=None, stats: bool = False, out_f32: bool = False,
                max_len: int | None = None) -> dict:
+        """Attention of one token per request.  The launch is sized by the table's width unless `max_len` gives a smaller bound on
+        the lengths (longer requests are cut off there): 1000 tokens of one request take 7.7 us under a bound of 1024 and
+        8.9 under one of 65536."""
         return K.decode8(q, self.k, self.v, self.k_scale, self.v_scale, scale, lens=self.lens, page_table=self.table,
                          max_len=max_len, plan=plan, stats=stats, out_f32=out_f32)
 

@@ -81,8 +81,12 @@ struct Decode8Launch {
 };
 // Blocks per warp up to which the short form is taken when its CTAs are most of the SMs, and when they are fewer.  The
 // lengths are on the device: with one bound on them for all, a longer form would leave SMs idle when they differ.
-// B200, us, general and short form, D 128, 8 KV heads: batch 1 / 1k 9.2 and 8.1, 4k 9.6 and 8.7, 8k 10.4 and 11.0; batch 4 / 4k
-// 13.7 and 11.6, batch 16 / 2k 19.5 and 16.5.
+// B200, us in a graph, general and short form, 8 KV heads: D 128, batch 1 / 1k 9.0 and 7.7, 4k 9.2 and 8.9, 8k 10.2 and 11.3; batch 4 /
+// 4k 12.9 and 12.1, batch 16 / 2k 19.1 and 17.0.  D 64, batch 1 / 1k 8.0 and 6.7, 4k 8.6 and 7.5, 8k 9.2 and 9.2, 12k 10.2 and
+// 10.4; batch 4 / 4k 11.0 and 9.1, batch 16 / 2k 13.6 and 11.7.
+// That the CTAs are at most as many as the SMs does not make them one wave: a cluster stays inside a GPC, and the GPCs do not
+// divide evenly.  16 to 18 heads in clusters of 8 take two (4k: 16.7 to 17.0, the general form 9.9 to 10.2), 36 and 37 heads
+// in clusters of 4 too (2k: 16.1 to 16.3, 10.2 to 10.3); 32 and 33 heads in clusters of 4 do not (8.8 and 8.9, 10.0).
 constexpr int kShortMost = 4, kShortFew = 2;
 template <int D, int MODE>
 Decode8Launch decode8_launch(const kvskip_decode8_params& p) {
@@ -90,7 +94,7 @@ Decode8Launch decode8_launch(const kvskip_decode8_params& p) {
   Decode8Launch l;
   l.ctas = static_cast<int>(std::min<int64_t>(kvb_host::num_sms(), items));
   l.warps = l.ctas * kvb::D8Cfg<D, MODE>::kWarps;
-  // the short form: as many CTAs per head as leave four blocks to each of them, in one wave
+  // the short form: as many CTAs per head as leave four blocks to each of them, no more than SMs in all
   constexpr int kWarps = kvb::D8Cfg<D, MODE>::kWarps;
   const int64_t heads = static_cast<int64_t>(p.B) * p.Hkv, longest = p.block_idx ? p.max_blocks : p.nb;
   int c = 1;
@@ -177,7 +181,9 @@ int launch_write8(const kvskip_write8_params& p, cudaStream_t s) {
 template <int KIND, int D, bool F16>
 int by_chunk(const kvskip_write8_params& p, cudaStream_t s) {
   // The slots of a warp: 64, or fewer where every warp of the GPU would not get a job, so that the tokens of a decode
-  // step spread over it.  B200, 256 tokens of 8 heads: 4.1 us with 4, 5.8 with 8; prompts of 54k tokens: 59 us with 64.
+  // step spread over it.  B200, us in a graph, 8 heads, with 4 and with 16: 64 tokens 3.1 and 9.1, 256 3.8 and 9.3, 512 6.0 and 9.3,
+  // 1024 10.3 and 9.4, 1700 15.0 and 9.5 (with 4 the last tokens wait for a place: 6 CTAs fit on an SM, one less than the grid
+  // counts on); prompts of 54k tokens with 64: 60.
   const int64_t warps = static_cast<int64_t>(kvb_host::num_sms()) * kvb::W8Cfg<D, 64>::kWarps, pairs = 2 * p.Hkv;
   if ((p.n + 63) / 64 * pairs >= warps) return launch_write8<KIND, D, F16, 64>(p, s);
   if ((p.n + 15) / 16 * pairs >= warps) return launch_write8<KIND, D, F16, 16>(p, s);

@@ -4,8 +4,8 @@
 // What bounds it: 2 D bytes per token and KV head against 4 G D operations, at most 32 operations a byte
 // for G = 16: HBM, as long as the arithmetic stays out of the way.  The codes go to the tensor cores as
 // fp16, which holds every e4m3 and int8 value exactly (converting q to 8 bits instead would lose what the
-// codes keep); q is held in fp16 relative to a power of two of its own row, so nothing of a bf16 q is
-// lost that could show in an fp32 sum.  M is the token (scores) or the channel (output) axis and the G
+// codes keep); q is held in fp16 relative to a power of two of its own row: exactly, bf16 values down to 2^-30 of the row's
+// largest, fp16 values down to 2^-27; a smaller one is rounded to a multiple of 2^-38 of it.  M is the token (scores) or the channel (output) axis and the G
 // query heads of a KV head are the 8 columns of mma.m16n8k16: the tcgen05 shapes start at 64 x 8 per
 // instruction but take A from shared memory or TMEM in fp16, so the converted codes would have to be
 // written back there first, which costs more than the products do.
@@ -40,6 +40,8 @@ struct D8Maps {
 // SMs (batch 16 / 64k in a loop of 0.3 s, under the power cap: 346 us with 7, 330 with 8, 372 with 10, 369 with 12; batch 1 /
 // 64k: 29.3, 29.5, 34.8, 40.5).  Fewer warps with two stages each are behind too, with one tile of columns at D 128 (6, 5 and 4
 // of them: 349, 375, 388 us for batch 16 / 64k; 34.3, 32.5, 31.9 for batch 1): a warp's own instructions become the bound.
+// D 64, whose tiles are half as large: 12 warps and 8 take 197 and 215 us for batch 16 / 64k in a loop (int8; 216 and 239 with 8
+// query heads), 22.8 and 21.5 for batch 1 / 64k, 7.1 and 6.6 for batch 1 / 1k.
 template <int D, int MODE>
 struct D8Cfg {
   static constexpr int kCols = MODE == 0 ? 4 : MODE == 1 ? 8 : 16;   // query heads there is room for
@@ -339,7 +341,7 @@ decode8_kernel(const __grid_constant__ kvskip_decode8_params p, const __grid_con
     return;
   }
   if (!SHORT && p.page_table) {
-    // the page table into L2 while the lengths are on their way (128 bytes a thread cover 7 MB of it)
+    // the page table into L2 while the lengths are on their way (128 bytes a thread: the first 4.8 MB of it with 8 warps)
     const int64_t at = (static_cast<int64_t>(blockIdx.x) * NT + tid) * 32;
     if (at < static_cast<int64_t>(p.B) * p.max_pages) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.page_table + at));
   }

@@ -419,7 +419,8 @@ def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | N
     Slots and positions: packed, request after request, in n_tokens places, or with per_row in a padded
     [B,per_row] list; -1 in places without a token.
     Returns dict(slots int64, positions int32, granted bool [B], lens, n_free); the last three are new tensors unless
-    granted_out / lens_out / n_free_out are given; the latter two may be lens and n_free themselves."""
+    granted_out / lens_out / n_free_out are given; the latter two may be lens and n_free themselves, nothing else that is
+    written may overlap another argument.  The new tensors of a call share one allocation: keeping one keeps them all."""
     if (n_tokens is None) == (per_row is None):
         raise ValueError("extend_pages: either n_tokens (packed) or per_row (padded)")
     if per_row is not None and per_row < 1:

@@ -719,6 +719,27 @@ def test_granted_and_positions_after_a_replay():
     assert cache.granted.tolist() == [True, False] and cache.lens.tolist() == [66, 64]
 
 
+def test_one_table_for_the_pools_of_several_layers():
+    """Slots, lengths and pages of one cache address another layer's pools too."""
+    B, Hkv, G, D = 3, 2, 4, 128
+    gen = torch.Generator().manual_seed(3)
+    cache = PagedKV8(8, B, Hkv, D, 256, DEV)
+    other = PagedKV8(8, B, Hkv, D, 256, DEV)                              # the same steps with tables of its own
+    k2, v2 = (torch.zeros_like(cache.k.view(torch.uint8)).view(cache.k.dtype) for _ in range(2))
+    ks2, vs2 = torch.ones_like(cache.k_scale), torch.ones_like(cache.v_scale)
+    new = torch.tensor([100, 0, 65], dtype=torch.int32, device=DEV)
+    x, y = (torch.randn(165, Hkv, D, generator=gen).to(torch.bfloat16).to(DEV) for _ in range(2))
+    slots = cache.extend(new, n_tokens=165)
+    cache.write(x, x, slots)
+    K.write8(y, x, slots, k2, v2, ks2, vs2)
+    other.write(y, x, other.extend(new, n_tokens=165))
+    q = torch.randn(B, Hkv * G, D, generator=gen).to(torch.bfloat16).to(DEV)
+    got = K.decode8(q, k2, v2, ks2, vs2, 0.1, lens=cache.lens, page_table=cache.table)
+    want = other.decode(q, 0.1)
+    assert torch.equal(got["out"], want["out"]) and torch.equal(got["lse"], want["lse"])
+    assert not torch.equal(cache.decode(q, 0.1)["out"], got["out"])
+
+
 def test_append_leaves_rows_without_a_request_alone():
     """After a release the row takes no page and no token until something is written for it."""
     B, Hkv, D = 4, 2, 64
