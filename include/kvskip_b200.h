@@ -378,7 +378,8 @@ typedef struct kvskip_write8_params {
 int kvskip_launch_write8(const kvskip_write8_params* p, void* stream);
 
 /* Page and slot tables from request lengths, on the device.  Request b holds lens[b] tokens in the pages
- * table[b, 0..ceil(lens[b]/64)) and is to get new_[b] more (negative counts as 0); free_pages
+ * table[b, 0..ceil(lens[b]/64)) and is to get new_[b] more (negative counts as 0; with live_only != 0, requests of length 0
+ * get none); free_pages
  * [num_free] is a stack of the free pages, *n_free of them.  In the order of the requests, every request
  * that fits (into max_pages pages, into the slot list, and into what the earlier ones left of the stack;
  * one that needs no page always fits into the stack, one without new tokens into any list) is granted: its new blocks get pages from the top
@@ -405,6 +406,7 @@ typedef struct kvskip_pages_params {
   int64_t n_tokens;
   int32_t per_row;
   int32_t B, max_pages, num_free;
+  int32_t live_only;    /* extend only */
 } kvskip_pages_params;
 int kvskip_launch_extend_pages(const kvskip_pages_params* p, void* stream);
 /* The pages of every request with done[b] != 0 go back on top of the stack (in the order of requests and

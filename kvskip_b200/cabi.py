@@ -77,7 +77,8 @@ class Write8Params(C.Structure):
 class PagesParams(C.Structure):
     _fields_ = [("lens", _vp), ("new_", _vp), ("done", _vp), ("table", _vp), ("free_pages", _vp), ("n_free", _vp),
                 ("lens_out", _vp), ("n_free_out", _vp), ("slots", _vp), ("positions", _vp), ("granted", _vp),
-                ("n_tokens", _i64), ("per_row", _i32), ("B", _i32), ("max_pages", _i32), ("num_free", _i32)]
+                ("n_tokens", _i64), ("per_row", _i32), ("B", _i32), ("max_pages", _i32), ("num_free", _i32),
+                ("live_only", _i32)]
 
 
 def _ptr(t):

@@ -205,15 +205,17 @@ class PagedKV8:
         self.positions = None
         self._ones = torch.ones(B, dtype=torch.int32, device=device)
 
-    def extend(self, new: torch.Tensor | None = None, *, n_tokens: int | None = None, per_row: int | None = None):
-        """Room for new[b] (int32 [B], default one in every row, rows of length 0 too) more tokens of every request;
-        returns their slots (see `kvskip.extend_pages`), `granted` and `positions` are kept on the object."""
+    def extend(self, new: torch.Tensor | None = None, *, n_tokens: int | None = None, per_row: int | None = None,
+               live_only: bool = False):
+        """Room for new[b] (int32 [B], default one in every row, rows of length 0 too unless live_only) more tokens of
+        every request; returns their slots (see `kvskip.extend_pages`), `granted` and `positions` are kept on the object."""
         if new is None:
             new = self._ones
         if n_tokens is None and per_row is None:
             per_row = 1
         r = K.extend_pages(self.lens, new, self.table, self.free_pages, self.n_free, n_tokens=n_tokens, per_row=per_row,
-                           lens_out=self.lens, n_free_out=self.n_free, granted_out=self.granted)
+                           lens_out=self.lens, n_free_out=self.n_free, granted_out=self.granted,
+                           live_only=live_only)
         self.positions = r["positions"]
         return r["slots"]
 
@@ -223,7 +225,7 @@ class PagedKV8:
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, new: torch.Tensor | None = None) -> None:
         """One token per request, [B,Hkv,D] each.  new (int32 [B] of 0 and 1): the rows that get one, a row without a
         request among them (which begins it); by default every row that holds a request, `lens[b] > 0`."""
-        slots = self.extend(self.lens.clamp(max=1) if new is None else new, per_row=1)
+        slots = self.extend(new, per_row=1, live_only=new is None)
         self.write(k_new.unsqueeze(2), v_new.unsqueeze(2), slots)
 
     def release(self, done: torch.Tensor) -> None:

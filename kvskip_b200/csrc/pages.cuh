@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(PG_THREADS) extend_pages_kernel(const __grid_c
     const int b = base + tid;
     int len = 0, add = 0;
     if (b < p.B) len = max(0, p.lens[b]), add = max(0, p.new_[b]);
+    if (p.live_only && len == 0) add = 0;
     const int64_t want_t = static_cast<int64_t>(len) + add;
     const int64_t want = (want_t + TILE - 1) / TILE;
     // One scan: whether the tokens of a request still fit into the list is known only behind it, but of the requests

@@ -953,7 +953,7 @@ std::vector<at::Tensor> extend_pages(const at::Tensor& lens, const at::Tensor& n
                                      const at::Tensor& free_pages, const at::Tensor& n_free, int64_t n_tokens,
                                      int64_t per_row, const c10::optional<at::Tensor>& lens_out,
                                      const c10::optional<at::Tensor>& n_free_out,
-                                     const c10::optional<at::Tensor>& granted_out) {
+                                     const c10::optional<at::Tensor>& granted_out, bool live_only) {
   TORCH_CHECK(lens.is_cuda(), "lens: contiguous CUDA int32");
   const c10::cuda::CUDAGuard guard(lens.device());
   TORCH_CHECK(lens.dim() == 1 && new_.numel() == lens.numel(), "new: [B]");
@@ -984,6 +984,7 @@ std::vector<at::Tensor> extend_pages(const at::Tensor& lens, const at::Tensor& n
   p.granted = static_cast<uint8_t*>(granted.data_ptr());
   p.n_tokens = n;
   p.per_row = static_cast<int32_t>(per_row);
+  p.live_only = live_only;
   raise_on(kvskip_launch_extend_pages(&p, cur_stream()));
   return {slots, positions, granted, lo, fo};
 }
@@ -1095,7 +1096,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("extend_pages", &extend_pages, "pages and slots for the new tokens of every request", py::arg("lens"),
         py::arg("new"), py::arg("page_table"), py::arg("free_pages"), py::arg("n_free"), py::arg("n_tokens") = 0,
         py::arg("per_row") = 0, py::arg("lens_out") = py::none(), py::arg("n_free_out") = py::none(),
-        py::arg("granted_out") = py::none());
+        py::arg("granted_out") = py::none(), py::arg("live_only") = false);
   m.def("release_pages", &release_pages, "pages of finished requests back to the free stack", py::arg("done"),
         py::arg("lens"), py::arg("page_table"), py::arg("free_pages"), py::arg("n_free"),
         py::arg("lens_out") = py::none(), py::arg("n_free_out") = py::none());

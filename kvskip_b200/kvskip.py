@@ -409,13 +409,14 @@ def _check_runs(slots) -> None:
 
 def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | None = None, per_row: int | None = None,
                  lens_out: torch.Tensor | None = None, n_free_out: torch.Tensor | None = None,
-                 granted_out: torch.Tensor | None = None) -> dict:
+                 granted_out: torch.Tensor | None = None, live_only: bool = False) -> dict:
     """Pages and slots for `new` int32 [B] more tokens of requests that hold `lens` int32 [B] tokens, built on
     the device without a host synchronisation.  Not in the reference, whose caller counts on the host.
 
     page_table int32 [B,max_pages] receives the pages of new blocks, taken from the top of the stack
     free_pages int32 [pages] with n_free int32 [1] entries.  A request that does not fit (into max_pages, into
-    the slot list, or into what earlier requests left of the stack) is refused as a whole.
+    the slot list, or into what earlier requests left of the stack) is refused as a whole.  live_only: requests of
+    length 0 get nothing, whatever `new` says.
     Slots and positions: packed, request after request, in n_tokens places, or with per_row in a padded
     [B,per_row] list; -1 in places without a token.
     Returns dict(slots int64, positions int32, granted bool [B], lens, n_free); the last three are new tensors unless
@@ -426,7 +427,7 @@ def extend_pages(lens, new, page_table, free_pages, n_free, *, n_tokens: int | N
     if per_row is not None and per_row < 1:
         raise ValueError("extend_pages: per_row >= 1")
     slots, positions, granted, lens2, n2 = (_EXT or ext()).extend_pages(lens, new, page_table, free_pages, n_free, n_tokens or 0,
-                                                              per_row or 0, lens_out, n_free_out, granted_out)
+                                                              per_row or 0, lens_out, n_free_out, granted_out, live_only)
     return {"slots": slots, "positions": positions, "granted": granted, "lens": lens2, "n_free": n2}
 
 

@@ -687,6 +687,19 @@ def test_extend_pages_grants_a_request_without_tokens_behind_a_full_list(B):
     assert torch.equal(table[:, 0].cpu(), torch.arange(B, dtype=torch.int32)) and (table[:, 1] == -1).all()
 
 
+@pytest.mark.parametrize("kw", [dict(per_row=2), dict(n_tokens=7)])
+def test_extend_pages_for_live_requests_only(kw):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    lens, new, free = [64, 0, 5, -2, 127], [1, 2, 2, 1, 2], [9, 8, 7, 6]
+    table = [[0, -1, -1], [-1] * 3, [1, -1, -1], [-1] * 3, [2, 3, -1]]
+    want = R.extend_ref(lens, [n if x > 0 else 0 for x, n in zip(lens, new)], table, free, 4, **kw)
+    td = i32(table)
+    r = K.extend_pages(i32(lens), i32(new), td, i32(free), i32([4]), live_only=True, **kw)
+    assert r["slots"].flatten().tolist() == want[0] and r["positions"].flatten().tolist() == want[1]
+    assert r["granted"].tolist() == want[2] and td.tolist() == want[4] and r["n_free"].tolist() == [want[5]]
+    assert r["lens"].tolist() == [max(0, x) for x in want[3]]
+
+
 def test_overlapping_tables_are_refused():
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
     lens, new, table, free, n = i32([3, 70]), i32([1, 1]), i32([[0, -1], [1, 2]]), i32([5, 4, 3]), i32([3])

@@ -193,7 +193,7 @@ def test_a_replayed_step_says_what_it_granted(monkeypatch):
     from kvskip_b200 import graph as G
 
     def extend_pages(lens, new, table, free, n_free, *, n_tokens=None, per_row=None, lens_out=None, n_free_out=None,
-                     granted_out=None):
+                     granted_out=None, live_only=False):
         granted = torch.empty(len(lens), dtype=torch.bool) if granted_out is None else granted_out
         n = len(lens) * per_row if per_row else n_tokens
         r = {"slots": torch.zeros(n, dtype=torch.int64), "positions": torch.full((n,), -1, dtype=torch.int32),
